@@ -479,6 +479,90 @@ typedef struct rsv_wkv_lora {
 } rsv_wkv_lora;
 int rsv_wkv7_lora_decode(rsv_ctx *ctx, const rsv_wkv_lora *op, uint64_t batch);
 
+/* ---- low-rank adapters of many requests beside a shared projection (no
+ * reference counterpart: it serves one set of weights).  Row t of a packed
+ * batch belongs to a request whose adapter is a = row_adapter[t]; every job
+ * adds that adapter's product to the row y of a shared projection (the output
+ * of rsv_gemm_ex, rsv_gemm_skinny, rsv_gemv_*):
+ *   out[t, :] = epi(y[t, :] + scale[a] * (x[t, :] A_a^T) B_a^T)
+ * with A_a = a[a, :R, :] and B_a = b[a, :, :R], R = min(ranks[a], rank).
+ * A row whose row_adapter is at or past n_adapter (0xFFFFFFFF by custom) has
+ * no adapter: out = epi(y).  What lies past an adapter's own rank R in a and b
+ * is never read into a result, whatever it holds.
+ *
+ * row_adapter U32 [rows], scale F32 [n_adapter] and ranks U32 [n_adapter]
+ * (0xFFFFFFFF: every adapter has the full rank) are read on the device, so a
+ * captured call follows what they hold when it is replayed.  Rows of one
+ * adapter may stand anywhere; any rows count from 1 on is one call: one
+ * decoded token per session, packed prompts, or both.  Rows that stand
+ * together share the adapter's reads.
+ *
+ * k, n and rank are multiples of 8 (16-byte fp16 rows), rank at most 128.
+ * epilogue: 0 (store) or 3 (relu^2), as rsv_gemm_ex.  out may be y itself;
+ * otherwise no job's out may be an operand of the call.  Products and sums
+ * are fp32 whatever the operands' types (an F16 out is rounded once).
+ * work: an F32 tensor of at least rsv_adapter_work floats, the caller's, used
+ * until the call's end on the stream (calls in flight at once on two lanes or
+ * contexts need one each).  1 to 8 jobs. */
+typedef struct rsv_adapter_job {
+    uint32_t a;   /* F16 [n_adapter, rank, k] */
+    uint32_t b;   /* F16 [n_adapter, n, rank] */
+    uint64_t n, k;
+    uint32_t x;   /* F32 or F16 [rows, k] */
+    uint32_t y;   /* F32 or F16 [rows, n] */
+    uint32_t out; /* F32 or F16 [rows, n] */
+    int epilogue;
+} rsv_adapter_job;
+int rsv_adapter_multi(rsv_ctx *ctx, const rsv_adapter_job *jobs, uint64_t njobs, uint32_t row_adapter,
+                      uint32_t scale, uint32_t ranks, uint64_t n_adapter, uint64_t rank, uint64_t rows,
+                      uint32_t work);
+/* Floats of work that rsv_adapter_multi needs for these jobs (only n and k
+ * are read; 0 if an argument is outside its limits). */
+uint64_t rsv_adapter_work(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows);
+
+/* ---- draws from given random numbers (no reference counterpart: its sampler
+ * hashes a seed and cuts the nucleus at 512 tokens).  Row b of logits
+ * [batch, n] (F32 or F16) with its own settings, filter[b] = {temperature,
+ * top_k bits, top_p, min_p} (F32 [batch, 4], written by rsv_store_filter or
+ * uploaded), and its own random number u = rand[b] (F32 [batch]):
+ *   e_i = exp((l_i - max l) / temperature); tokens are ranked by logit, equal
+ *   logits by index;
+ *   top_k: the first top_k tokens stay (0 or >= n: all);
+ *   min_p: of these, those with e_i >= min_p;
+ *   top_p: of these, each token before which less than top_p of their sum has
+ *   gone by (>= 1: all; the first token always stays);
+ *   the draw: the first token in index order at which the running sum of the
+ *   kept e passes u times their whole sum.
+ * temperature <= 0 or NaN: the largest logit.  u is taken into [0, 1] (NaN: 0;
+ * 1: the last kept token).  A NaN logit counts as -inf; -inf is never drawn;
+ * +inf logits share the row among themselves.  A row without any token left
+ * gives token 0xFFFFFFFF (which the gather entry points read as a row of
+ * zeros) and logp -inf.  top_p or min_p NaN: no cut; min_p above 1 is 1.
+ * logp[b] (F32 [batch], or 0xFFFFFFFF for none) is the logarithm of the
+ * probability that the token had among the kept ones (0 where greedy).
+ * Sums are exact: weights are integers with 62 - ceil(log2 n) bits after the
+ * point, so a row's draw depends on nothing but its logits, settings and u:
+ * not on its place in the batch, nor on how the work is split.
+ * 1 <= n <= 1048576.  work: an F32 tensor of at least rsv_logits_work floats,
+ * the caller's, as for rsv_adapter_multi. */
+int rsv_sample_rand_batch(rsv_ctx *ctx, uint32_t logits, uint32_t token, uint64_t n, uint32_t filter,
+                          uint32_t rand, uint32_t logp, uint32_t work, uint64_t batch);
+/* filter[row] = the four settings, stream-ordered (as rsv_store_sampler). */
+int rsv_store_filter(rsv_ctx *ctx, uint32_t filter, uint64_t row, float temperature, uint32_t top_k, float top_p,
+                     float min_p);
+/* ---- log-probabilities of given tokens (no reference counterpart: a host
+ * downloads the rows, gpu_model.rs:3784-3794).  For each row of logits
+ * [rows, n] (F32 or F16): logp = l[token] - ln sum_i exp(l_i), and rank (U32,
+ * or 0xFFFFFFFF for none) the number of tokens ahead of it (a larger logit, or
+ * an equal one at a lower index: 0 is what argmax gives).  A token at or past
+ * n (0xFFFFFFFF by custom) asks for nothing: logp 0, rank 0, the row is not
+ * read.  NaN logits count as -inf; a token of -inf has logp -inf.  Limits and
+ * work as rsv_sample_rand_batch. */
+int rsv_token_logprobs(rsv_ctx *ctx, uint32_t logits, uint32_t token, uint64_t n, uint32_t logp, uint32_t rank,
+                       uint32_t work, uint64_t rows);
+/* Floats of work that the two calls above need (0 outside their limits). */
+uint64_t rsv_logits_work(uint64_t n, uint64_t rows);
+
 /* ---- profiling hooks (backend.rs:67-70); kernel timing is done with rocprofv3 */
 int rsv_clear_kernel_prof(rsv_ctx *ctx);
 int rsv_dump_kernel_prof(rsv_ctx *ctx);

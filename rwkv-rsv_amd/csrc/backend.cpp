@@ -1744,3 +1744,168 @@ extern "C" int rsv_tile_weights(rsv_ctx *ctx, uint32_t src, uint64_t n, uint64_t
     *out = id;
     return 0;
 }
+
+// ------------------------------------- adapters, draws, log-probabilities
+// An F32 or F16 operand of at least min_len elements.
+static int real_opnd(rsv_ctx *ctx, uint32_t id, uint64_t min_len, void **p, int *f16, const char *what) {
+    Tensor *t = get_tensor(ctx, id);
+    if (t && t->dtype == RSV_U32) return RSV_FAIL("%s: tensor %u must be F32 or F16", what, id);
+    if (opnd(ctx, id, -1, min_len, p, what)) return -1;
+    *f16 = t->dtype == RSV_F16;
+    return 0;
+}
+
+constexpr uint64_t kAdapterRows = (uint64_t)1 << 20, kAdapterDim = (uint64_t)1 << 24, kAdapterRank = 128;
+
+// The limits of rsv_adapter_multi that do not need a context.
+static int adapter_limits(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows) {
+    if (!jobs || njobs == 0 || njobs > (uint64_t)kMaxJobs) return RSV_FAIL("adapter_multi: 1..%d jobs", kMaxJobs);
+    if (rank == 0 || rank > kAdapterRank || rank % 8)
+        return RSV_FAIL("adapter_multi: rank %llu is not a multiple of 8 in 8..%llu", (unsigned long long)rank,
+                        (unsigned long long)kAdapterRank);
+    if (rows == 0 || rows > kAdapterRows) return RSV_FAIL("adapter_multi: rows %llu outside 1..%llu", (unsigned long long)rows, (unsigned long long)kAdapterRows);
+    for (uint64_t i = 0; i < njobs; i++) {
+        const rsv_adapter_job &q = jobs[i];
+        if (q.n == 0 || q.k == 0 || q.n % 8 || q.k % 8 || q.n > kAdapterDim || q.k > kAdapterDim)
+            return RSV_FAIL("adapter_multi job %llu: n=%llu, k=%llu must be multiples of 8 up to %llu",
+                            (unsigned long long)i, (unsigned long long)q.n, (unsigned long long)q.k,
+                            (unsigned long long)kAdapterDim);
+        if (q.epilogue != GE_STORE && q.epilogue != GE_RELU2)
+            return RSV_FAIL("adapter_multi job %llu: epilogue %d is not 0 (store) or 3 (relu^2)", (unsigned long long)i, q.epilogue);
+    }
+    return 0;
+}
+
+extern "C" uint64_t rsv_adapter_work(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows) {
+    if (adapter_limits(jobs, njobs, rank, rows)) return 0;
+    return adapter_work_words(jobs, njobs, rank, rows);
+}
+
+extern "C" int rsv_adapter_multi(rsv_ctx *ctx, const rsv_adapter_job *jobs, uint64_t njobs, uint32_t row_adapter,
+                                 uint32_t scale, uint32_t ranks, uint64_t n_adapter, uint64_t rank, uint64_t rows,
+                                 uint32_t work) {
+    CHECK_CTX();
+    if (adapter_limits(jobs, njobs, rank, rows)) return -1;
+    if (n_adapter == 0 || n_adapter > kAdapterRows)
+        return RSV_FAIL("adapter_multi: n_adapter %llu outside 1..%llu", (unsigned long long)n_adapter, (unsigned long long)kAdapterRows);
+    AdapterJobs J{};
+    J.njob = (int)njobs;
+    J.n_adapter = (int)n_adapter;
+    J.rank = (int)rank;
+    J.rows = (int)rows;
+    OPND(ra, row_adapter, RSV_U32, rows, "adapter_multi row_adapter");
+    J.row_adapter = U32P(ra);
+    OPND(sc, scale, RSV_F32, n_adapter, "adapter_multi scale");
+    J.scale = F32P(sc);
+    if (ranks != 0xFFFFFFFFu) {
+        OPND(rk, ranks, RSV_U32, n_adapter, "adapter_multi ranks");
+        J.ranks = U32P(rk);
+    }
+    OPND(wk, work, RSV_F32, adapter_work_words(jobs, njobs, rank, rows), "adapter_multi work");
+    for (uint64_t i = 0; i < njobs; i++) {
+        const rsv_adapter_job &q = jobs[i];
+        AdapterJob &d = J.j[i];
+        void *p = nullptr;
+        int f16 = 0;
+        if (opnd(ctx, q.a, RSV_F16, n_adapter * rank * q.k, &p, "adapter_multi a")) return -1;
+        d.a = (const _Float16 *)p;
+        if (opnd(ctx, q.b, RSV_F16, n_adapter * q.n * rank, &p, "adapter_multi b")) return -1;
+        d.b = (const _Float16 *)p;
+        if (real_opnd(ctx, q.x, rows * q.k, &p, &f16, "adapter_multi x")) return -1;
+        d.x = p, d.x16 = f16;
+        if (real_opnd(ctx, q.y, rows * q.n, &p, &f16, "adapter_multi y")) return -1;
+        d.y = p, d.y16 = f16;
+        if (real_opnd(ctx, q.out, rows * q.n, &p, &f16, "adapter_multi out")) return -1;
+        d.out = p, d.o16 = f16;
+        d.n = (int)q.n;
+        d.k = (int)q.k;
+        d.epi = q.epilogue;
+    }
+    // what a block writes, no other block reads or writes
+    for (uint64_t i = 0; i < njobs; i++) {
+        const uint32_t o = jobs[i].out;
+        bool clash = o == row_adapter || o == scale || o == ranks || o == work;
+        for (uint64_t l = 0; l < njobs; l++)
+            clash = clash || o == jobs[l].a || o == jobs[l].b || o == jobs[l].x || work == jobs[l].a ||
+                    work == jobs[l].b || work == jobs[l].x || work == jobs[l].y ||
+                    (l != i && (o == jobs[l].y || o == jobs[l].out));
+        if (clash || work == row_adapter || work == scale || work == ranks)
+            return RSV_FAIL("adapter_multi job %llu: out or work is another operand of the call (out may be its own y)", (unsigned long long)i);
+    }
+    return launch_adapter(ctx, J, F32P(wk));
+}
+
+static int logits_limits(uint64_t n, uint64_t rows, const char *what) {
+    if (n == 0 || n > kLogitsMaxN)
+        return RSV_FAIL("%s: n=%llu outside 1..%llu", what, (unsigned long long)n, (unsigned long long)kLogitsMaxN);
+    if (rows == 0 || rows > kAdapterRows)
+        return RSV_FAIL("%s: %llu rows outside 1..%llu", what, (unsigned long long)rows, (unsigned long long)kAdapterRows);
+    return 0;
+}
+
+extern "C" uint64_t rsv_logits_work(uint64_t n, uint64_t rows) {
+    return logits_limits(n, rows, "logits_work") ? 0 : logits_work_words(n, rows);
+}
+
+// Outputs (the first nout ids) and inputs of a call: no output may be another operand.
+static int distinct_outputs(const uint32_t *ids, int nout, int n, const char *what) {
+    for (int o = 0; o < nout; o++)
+        for (int i = 0; i < n; i++)
+            if (i != o && ids[o] != 0xFFFFFFFFu && ids[o] == ids[i])
+                return RSV_FAIL("%s: tensor %u is an output and another operand", what, ids[o]);
+    return 0;
+}
+
+extern "C" int rsv_sample_rand_batch(rsv_ctx *ctx, uint32_t logits, uint32_t token, uint64_t n, uint32_t filter,
+                                     uint32_t rand, uint32_t logp, uint32_t work, uint64_t batch) {
+    CHECK_CTX();
+    if (logits_limits(n, batch, "sample_rand")) return -1;
+    void *l = nullptr;
+    int f16 = 0;
+    if (real_opnd(ctx, logits, n * batch, &l, &f16, "sample_rand logits")) return -1;
+    OPND(t, token, RSV_U32, batch, "sample_rand token");
+    OPND(f, filter, RSV_F32, 4 * batch, "sample_rand filter");
+    OPND(u, rand, RSV_F32, batch, "sample_rand rand");
+    OPND(w, work, RSV_F32, logits_work_words(n, batch), "sample_rand work");
+    float *lp = nullptr;
+    if (logp != 0xFFFFFFFFu) {
+        OPND(p, logp, RSV_F32, batch, "sample_rand logp");
+        lp = F32P(p);
+    }
+    const uint32_t ids[6] = {token, logp, work, logits, filter, rand};
+    if (distinct_outputs(ids, 3, 6, "sample_rand")) return -1;
+    return launch_draw(ctx, l, f16, U32P(t), n, F32P(f), F32P(u), lp, F32P(w), batch);
+}
+
+extern "C" int rsv_store_filter(rsv_ctx *ctx, uint32_t filter, uint64_t row, float temperature, uint32_t top_k,
+                                float top_p, float min_p) {
+    CHECK_CTX();
+    if (row >= kAdapterRows) return RSV_FAIL("store_filter: row %llu", (unsigned long long)row);
+    OPND(f, filter, RSV_F32, 4 * (row + 1), "store_filter");
+    uint32_t words[4];
+    memcpy(&words[0], &temperature, 4);
+    words[1] = top_k;
+    memcpy(&words[2], &top_p, 4);
+    memcpy(&words[3], &min_p, 4);
+    return launch_set_u32(ctx, U32P(f) + 4 * row, words, 4);
+}
+
+extern "C" int rsv_token_logprobs(rsv_ctx *ctx, uint32_t logits, uint32_t token, uint64_t n, uint32_t logp,
+                                  uint32_t rank, uint32_t work, uint64_t rows) {
+    CHECK_CTX();
+    if (logits_limits(n, rows, "token_logprobs")) return -1;
+    void *l = nullptr;
+    int f16 = 0;
+    if (real_opnd(ctx, logits, n * rows, &l, &f16, "token_logprobs logits")) return -1;
+    OPND(t, token, RSV_U32, rows, "token_logprobs token");
+    OPND(p, logp, RSV_F32, rows, "token_logprobs logp");
+    OPND(w, work, RSV_F32, logits_work_words(n, rows), "token_logprobs work");
+    uint32_t *rk = nullptr;
+    if (rank != 0xFFFFFFFFu) {
+        OPND(r, rank, RSV_U32, rows, "token_logprobs rank");
+        rk = U32P(r);
+    }
+    const uint32_t ids[5] = {logp, rank, work, logits, token};
+    if (distinct_outputs(ids, 3, 5, "token_logprobs")) return -1;
+    return launch_logprobs(ctx, l, f16, U32P(t), n, F32P(p), rk, F32P(w), rows);
+}

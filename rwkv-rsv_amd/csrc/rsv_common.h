@@ -302,6 +302,30 @@ struct WkvLoraArgs {
     float eps, gn_eps;
 };
 int launch_wkv7_lora(rsv_ctx *ctx, const WkvLoraArgs &a, int batch);
+// Per-request low-rank adapters (k_adapter.hip).
+struct AdapterJob {
+    const _Float16 *a, *b;  // [n_adapter, rank, k], [n_adapter, n, rank]
+    const void *x, *y;      // [rows, k], [rows, n], F32 or F16
+    void *out;              // [rows, n], F32 or F16
+    float *h;               // [rows, rank] of the work area (filled by the launcher)
+    int n, k;
+    int x16, y16, o16, epi;  // epi: GE_STORE or GE_RELU2
+};
+struct AdapterJobs {
+    AdapterJob j[kMaxJobs];
+    const uint32_t *row_adapter, *ranks;  // [rows]; [n_adapter] or null
+    const float *scale;                   // [n_adapter]
+    int njob, n_adapter, rank, rows;
+};
+uint64_t adapter_work_words(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows);
+int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work);
+// Draws and log-probabilities from logits rows (k_logits.hip).
+constexpr uint64_t kLogitsMaxN = (uint64_t)1 << 20;
+uint64_t logits_work_words(uint64_t n, uint64_t rows);
+int launch_draw(rsv_ctx *ctx, const void *logits, int f16, uint32_t *token, uint64_t n, const float *filter,
+                const float *rnd, float *logp, float *work, uint64_t rows);
+int launch_logprobs(rsv_ctx *ctx, const void *logits, int f16, const uint32_t *token, uint64_t n, float *logp,
+                    uint32_t *rank, float *work, uint64_t rows);
 // Sparse ffn.value (k_sparse.hip): tiled fp16 copy and x += r2 V over non-zero r2.
 int launch_tile_ffn_value(rsv_ctx *ctx, const uint8_t *idx, const uint32_t *sz, const _Float16 *w16, _Float16 *out,
                           int c, int fh);

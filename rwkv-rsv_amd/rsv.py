@@ -61,6 +61,12 @@ class MmJob(ctypes.Structure):
                 ("scale", ctypes.c_uint32), ("tiled", ctypes.c_int)]
 
 
+class AdapterJob(ctypes.Structure):
+    """rsv_adapter_job (include/rsv_hip.h)."""
+    _fields_ = [("a", ctypes.c_uint32), ("b", ctypes.c_uint32), ("n", ctypes.c_uint64), ("k", ctypes.c_uint64),
+                ("x", ctypes.c_uint32), ("y", ctypes.c_uint32), ("out", ctypes.c_uint32), ("epilogue", ctypes.c_int)]
+
+
 def _ctype(decl):
     d = decl.replace("const", "").strip()
     ptr = d.count("*")
@@ -76,7 +82,7 @@ def _ctype(decl):
     if base == "rsv_int8":
         return ctypes.POINTER(Int8Handle)
     if base in ("rsv_model_info", "rsv_sampler_params", "rsv_gemv_job", "rsv_mm_job", "rsv_serve_step",
-                "rsv_wkv_lora"):
+                "rsv_wkv_lora", "rsv_adapter_job"):
         return ctypes.c_void_p
     return ctypes.POINTER(scalars[base])
 

@@ -19,7 +19,7 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", INC, "-I
 COMMON += os.environ.get("RSV_EXTRA_FLAGS", "").split()
 
 BACKEND_SRCS = ["backend.cpp", "k_gemv.hip", "k_wkv.hip", "k_misc.hip", "k_sample.hip", "k_gemm.hip",
-                "k_skinny.hip", "k_sparse.hip"]
+                "k_skinny.hip", "k_sparse.hip", "k_adapter.hip", "k_logits.hip"]
 HOST_SRCS = ["host.cpp"]
 
 

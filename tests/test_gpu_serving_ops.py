@@ -260,9 +260,9 @@ def test_adapters_replayed(be, tens):
 def test_adapters_refusals(be, tens):
     import rsv
     rng = np.random.default_rng(0)
-    c = Adapters(tens, rng, 4, 2, 16, [(64, 32), (64, 32)], "f16").upload()
+    c = Adapters(tens, rng, 70, 2, 16, [(64, 32), (64, 32)], "f16").upload()
     args = lambda **o: [o.get("jobs", c.jobs), o.get("njobs", 2), o.get("ids", c.t_ids), o.get("scale", c.t_scale),  # noqa: E731
-                        o.get("ranks", c.t_ranks), o.get("na", 2), o.get("rank", 16), o.get("rows", 4), o.get("work", c.work)]
+                        o.get("ranks", c.t_ranks), o.get("na", 2), o.get("rank", 16), o.get("rows", 70), o.get("work", c.work)]
     def job(i=0, **f):
         js = (rsv.AdapterJob * 2)(*[rsv.AdapterJob(*[getattr(j, n) for n, _ in j._fields_]) for j in c.jobs])
         for n, v in f.items():
@@ -272,7 +272,7 @@ def test_adapters_refusals(be, tens):
     for match, bad in [
             ("1..8 jobs", dict(njobs=0)), ("1..8 jobs", dict(njobs=9)), ("1..8 jobs", dict(jobs=None)),
             ("rank 0", dict(rank=0)), ("rank 12", dict(rank=12)), ("rank 136", dict(rank=136)),
-            ("rows 0", dict(rows=0)), ("rows 1048577", dict(rows=1048577)), ("needs", dict(rows=5)),
+            ("rows 0", dict(rows=0)), ("rows 1048577", dict(rows=1048577)), ("needs", dict(rows=71)),
             ("n_adapter 0", dict(na=0)), ("needs", dict(na=3)), ("unknown tensor", dict(ids=9999999)),
             ("unknown tensor", dict(scale=NONE)), ("needs", dict(work=c.t_scale)), ("unknown tensor", dict(work=NONE)),
             ("multiples of 8", dict(jobs=job(n=0))), ("multiples of 8", dict(jobs=job(k=60))),
@@ -282,7 +282,7 @@ def test_adapters_refusals(be, tens):
             ("another operand", dict(jobs=job(out=j1.y))), ("another operand", dict(jobs=job(1, out=j0.x))),
             ("another operand", dict(jobs=job(y=c.work, out=c.t_out[0]), work=c.work))]:
         if match == "another operand" and "work" in bad:
-            big = tens(n=4096)
+            big = tens(n=1 << 20)
             bad = dict(jobs=job(y=big), work=big)
         with pytest.raises(rsv.RsvError, match=match):
             be.call("rsv_adapter_multi", *args(**bad))

@@ -2,6 +2,7 @@
 // numbers (rsv_sample_rand_batch) and log-probabilities of given tokens
 // (rsv_token_logprobs).
 #include <algorithm>
+#include <type_traits>
 
 #include "rsv_common.h"
 
@@ -47,35 +48,47 @@ __device__ __forceinline__ void lg_unpack(uint4 q, float (&v)[F16 ? 8 : 4]) {
 // token from that piece alone.  So the row is read once, and then what lies in
 // one bin and one piece.
 //
-// A token's weight is 2^x, x = l * log2(e) / T, held as an integer with 48 bits
-// below the octave E above the piece's largest (E - x > 0).  With c = 64
-// log2(e) / T, q = floor(l c) and r = l c - q (one rounding) the weight is
-// 2^(q/64) 2^(r/64): a 64-entry table and a Taylor polynomial of degree 5 in
-// r ln2 / 64 < 0.011 (2e-15 off).  Adding 2^52 to the scaled weight leaves the
-// integer in the low bits of the sum.  Integers add up the same in any order;
-// pieces are put together in 64-bit floats in the pieces' order, which
-// depends on n alone.  Bins follow q, so they mean the same in every piece.
+// A token's weight is 2^x, x = l log2(e) / T, held as an integer with `bits`
+// bits below E, a whole octave above the piece's largest x.  With c = 1024
+// log2(e) / T: q = l c rounded to an integer (adding 1.5 2^52 leaves it in the
+// sum's low bits, right for |l c| < 2^51), r = l c - q in one rounding, and
+//   2^x = 2^(q >> 10) tab[q & 1023] (1 + r ln2/1024 + ...),
+// a Taylor polynomial of degree 3 in an argument below 3.4e-4 (6e-16 off).
+// Adding 2^52 to the scaled weight leaves the integer in the low bits.  Eight
+// 64-bit float operations a token; exp() takes about four times as many.
+// Integers add up the same in any order; pieces are put together in 64-bit
+// floats in the pieces' order, which depends on n alone.  Bins follow q, so
+// they mean the same in every piece.
+//
+// Tokens 36.5 T and more below a piece's maximum (2^-52) have no weight and
+// stand in no bin.  Rows that are only settled by their maximum (+inf, or
+// |l c| past 2^50, where different logits are 36 T apart) are `sharp`: tokens
+// at the maximum weigh 2^(bits - 1), the others nothing.
 constexpr int kPiece = 8192, kDrawThreads = 1024, kPer = kPiece / kDrawThreads;
-constexpr int kBins = 512, kBits = 48, kMaxPieces = (int)(kLogitsMaxN / kPiece);
-constexpr int kList = 4096;  // a bin's tokens held in LDS
+constexpr int kBins = 512, kSteps = 1024, kBinShift = 7, kMaxPieces = (int)(kLogitsMaxN / kPiece);
+constexpr int kSharpDown = kSteps - 1;  // a sharp maximum stands in its first octave's last bin
+constexpr int kDeepBin = 50 * 8;  // from here on weights vanish beside the maximum's
+constexpr int kPlainBits = 48;    // weights of a row without cuts
+constexpr int kCutBits = 37;      // with cuts: a bin packs its sum (8192 2^37 = 2^50) and above it its count
+constexpr int kInBits = 40;       // inside a bin, below the bin's octave: up to 2^20 tokens
+constexpr uint64_t kSumMask = ((uint64_t)1 << 50) - 1;
+constexpr int kList = 4096;       // a bin's tokens held in LDS
 
 struct DrawPiece {
     float m;        // largest logit (-inf: nothing to draw)
-    uint32_t idx;   // its lowest token
-    double e64;     // 64 E
-    uint64_t sum;
-    uint32_t cnt, pad;  // tokens in the histogram
+    uint32_t idx;   // its lowest token (greedy rows)
+    double e;       // 1024 E
+    uint64_t sum;   // plain rows
 };
 struct DrawWork {
     DrawPiece *piece;   // [rows, P]
-    uint64_t *sum;      // [rows, P, kBins]
-    uint16_t *cnt;      // [rows, P, kBins]
+    uint64_t *hist;     // [rows, P, kBins]
 };
 struct DrawRow {
-    double T, c64;
-    float min_p;    // > 0: active
+    double T, c;
+    float min_p;     // > 0: active
     uint32_t top_k;  // > 0 and < n: active
-    float top_p;    // < 1: active
+    float top_p;     // < 1: active
     bool greedy, cuts;
 };
 
@@ -85,7 +98,7 @@ __device__ __forceinline__ DrawRow draw_row(const float *f, int n) {
     const uint32_t k = __float_as_uint(f[1]);
     d.greedy = !(T > 0.0f);
     d.T = T;
-    d.c64 = 64.0 * 1.4426950408889634074 / (double)T;
+    d.c = kSteps * 1.4426950408889634074 / (double)T;
     d.top_k = k < (uint32_t)n ? k : 0;
     d.top_p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;
     d.min_p = m > 0.0f && T < INFINITY ? fminf(m, 1.0f) : 0.0f;
@@ -93,39 +106,51 @@ __device__ __forceinline__ DrawRow draw_row(const float *f, int n) {
     return d;
 }
 
-// 64 E of a piece (or its inf tokens): whole octaves strictly above its maximum.
 constexpr double kInfE = 1e300;
-__device__ __forceinline__ double draw_e64(float m, double c64) {
-    return m == INFINITY ? kInfE : 64.0 * (floor(floor((double)m * c64) * 0.015625) + 1.0);
+constexpr double kRound = 6755399441055744.0;  // 1.5 2^52
+__device__ __forceinline__ bool draw_sharp(float m, double c) { return m == INFINITY || fabs((double)m * c) >= 1125899906842624.0; }
+__device__ __forceinline__ double draw_e(float m, double c) {
+    return m == INFINITY ? kInfE : kSteps * (floor(rint((double)m * c) * (1.0 / kSteps)) + 1.0);
 }
-// q of a token in a piece with this maximum; +inf tokens stand one step below
-// kInfE, the others of such a piece carry no weight.
-__device__ __forceinline__ double draw_q(float l, double c64, bool inf) {
-    return inf ? l == INFINITY ? kInfE : -kInfE : floor((double)l * c64);
+// The logit from which tokens carry weight beside a maximum m; -inf never does.
+constexpr float kLeast = -3.402823466e38f;
+__device__ __forceinline__ float draw_low(float m, const DrawRow &d) {
+    return m == INFINITY ? m : fmaxf((float)((double)m - 36.5 * d.T), kLeast);
 }
-// A token's bin below the piece's octave: 0 .. kBins - 1, the last one open.
-__device__ __forceinline__ int draw_bin(double q, double e64) {
-    const double down = e64 - 1.0 - q;  // 0, 1, ...
-    return down < (double)(8 * kBins) ? max((int)down, 0) >> 3 : kBins - 1;
-}
-// r of a token; where a step is no longer seen beside l c (|l c| > 2^53),
-// tokens of different logits are whole octaves apart and any r will do
-__device__ __forceinline__ double draw_frac(float l, double c64, double q) {
-    return fmin(fmax(fma((double)l, c64, -q), 0.0), 1.0);
-}
-__device__ __forceinline__ uint64_t draw_weight(float l, double c64, double q, double e64, bool inf, const double *tab) {
-    const double down = e64 - q;
-    if (!(down < 64.0 * kBits + 64.0)) return 0;
-    if (inf) return 1ull << (kBits - 1);
-    const int k = -(int)down;  // -64 kBits - 63 .. 0
-    const double r = draw_frac(l, c64, q) * (0.69314718055994530942 / 64.0);
-    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    const double t = ldexp(tab[k & 63], (k >> 6) + kBits);
+
+// What weights are taken against: a piece's octave or a bin's.
+struct DrawUnit {
+    double c;
+    uint32_t e;      // low word of E + kRound
+    float m;         // sharp: the one logit that weighs
+    bool sharp;
+    __device__ DrawUnit(double c_, double e_, float m_) : c(c_), e((uint32_t)__double_as_longlong(e_ + kRound)), m(m_), sharp(draw_sharp(m_, c_)) {}
+    // q - E, at most 0 (and not below -60 octaves, where nothing is left to weigh)
+    __device__ int steps(float l, double &r) const {
+        const double t = fma((double)l, c, kRound);
+        r = fma((double)l, c, kRound - t);
+        return max((int)((uint32_t)__double_as_longlong(t) - e), -60 * kSteps);
+    }
+};
+__device__ __forceinline__ uint64_t draw_value(int k, double r, int bits, const double *tab) {
+    constexpr double a1 = 0.69314718055994530942 / kSteps, a2 = a1 * a1 / 2.0, a3 = a2 * a1 / 3.0;
+    const double p = fma(r, fma(r, fma(r, a3, a2), a1), 1.0);
+    const double t = __longlong_as_double(__double_as_longlong(tab[k & (kSteps - 1)]) + ((int64_t)((k >> 10) + bits) << 52));
     return (uint64_t)__double_as_longlong(fma(t, p, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+}
+// A token's weight; l at or above draw_low of the unit's maximum.
+__device__ __forceinline__ uint64_t draw_weight(const DrawUnit &u, float l, int bits, const double *tab, int &down) {
+    if (u.sharp) {
+        down = kSharpDown;
+        return l == u.m ? 1ull << (bits - 1) : 0;
+    }
+    double r;
+    const int k = u.steps(l, r);
+    down = -k;
+    return draw_value(k, r, bits, tab);
+}
+__device__ __forceinline__ void draw_table(double *tab) {
+    for (int i = threadIdx.x; i < kSteps; i += kDrawThreads) tab[i] = exp2((double)i / kSteps);
 }
 
 template <typename T>
@@ -165,21 +190,20 @@ __device__ __forceinline__ void piece_load(const void *logits, size_t base, int 
 template <bool F16>
 __global__ __launch_bounds__(kDrawThreads) void k_draw_scan(const void *__restrict__ logits, int n, int P, bool aligned,
                                                             const float *__restrict__ filter, DrawWork W) {
-    __shared__ double tab[64];
+    __shared__ double tab[kSteps];
+    __shared__ uint64_t hist[kBins];
+    __shared__ uint64_t ss[16];
     __shared__ float sm[16];
     __shared__ uint32_t si[16];
-    __shared__ uint64_t ss[16];
-    __shared__ uint64_t hsum[kBins];
-    __shared__ uint32_t hcnt[kBins];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t row = blockIdx.x / P;
     const int p = blockIdx.x % P, i0 = p * kPiece;
     float v[kPer];
     piece_load<F16>(logits, row * n, i0, n, aligned, v);
     const DrawRow d = draw_row(filter + 4 * row, n);
-    if (tid < 64) tab[tid] = exp2((double)tid / 64.0);
+    if (!d.greedy) draw_table(tab);
     if (d.cuts)
-        for (int b = tid; b < kBins; b += kDrawThreads) hsum[b] = 0, hcnt[b] = 0;
+        for (int b = tid; b < kBins; b += kDrawThreads) hist[b] = 0;
     float m = v[0];
 #pragma unroll
     for (int e = 1; e < kPer; e++) m = fmaxf(m, v[e]);
@@ -187,8 +211,9 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_scan(const void *__restri
     if (lane == 0) sm[wave] = m;
     __syncthreads();
     for (int w = 0; w < 16; w++) m = fmaxf(m, sm[w]);
-    uint32_t idx = 0xFFFFFFFFu;
+    DrawPiece *out = W.piece + row * P + p;
     if (d.greedy) {
+        uint32_t idx = 0xFFFFFFFFu;
 #pragma unroll
         for (int e = kPer - 1; e >= 0; e--)
             if (v[e] == m) idx = i0 + piece_token<F16>(aligned, e);
@@ -196,49 +221,48 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_scan(const void *__restri
         if (lane == 0) si[wave] = idx;
         __syncthreads();
         for (int w = 0; w < 16; w++) idx = min(idx, si[w]);
+        if (tid == 0) *out = DrawPiece{m, idx, 0.0, 0};
+        return;
     }
-    DrawPiece *out = W.piece + row * P + p;
-    const bool inf = m == INFINITY;
-    const double e64 = draw_e64(m, d.c64);
-    if (d.greedy || m == -INFINITY) {
-        if (tid == 0) *out = DrawPiece{m, idx, m == -INFINITY ? -kInfE : e64, 0, 0, 0};
-        if (d.greedy) return;
+    if (m == -INFINITY) {
+        if (tid == 0) *out = DrawPiece{m, 0, -kInfE, 0};
+        return;
     }
+    const double e = draw_e(m, d.c);
+    const DrawUnit unit(d.c, e, m);
+    float low = draw_low(m, d);
     // below this nothing survives min-p, whatever the row's maximum
-    const float low = d.min_p > 0.0f ? (float)((double)m + d.T * log((double)d.min_p)) : -INFINITY;
-    const float floor_l = low - fabsf(low) * 2.4e-7f;
-    uint64_t s = 0;
-    uint32_t c = 0;
-    if (m > -INFINITY) {
-#pragma unroll
-        for (int e = 0; e < kPer; e++) {
-            if (v[e] == -INFINITY || (d.min_p > 0.0f && v[e] < floor_l)) continue;
-            const double q = draw_q(v[e], d.c64, inf);
-            const uint64_t w = draw_weight(v[e], d.c64, q, e64, inf, tab);
-            s += w;
-            c++;
-            if (d.cuts) {
-                const int b = draw_bin(q, e64);
-                atomicAdd((unsigned long long *)&hsum[b], (unsigned long long)w);
-                atomicAdd(&hcnt[b], 1u);
-            }
-        }
-        s = wave_sum(s);
-        c = wave_sum(c);
-        if (lane == 0) ss[wave] = s, si[wave] = c;
-    }
-    __syncthreads();
-    if (tid == 0 && m > -INFINITY) {
-        s = 0;
-        c = 0;
-        for (int w = 0; w < 16; w++) s += ss[w], c += si[w];
-        *out = DrawPiece{m, idx, e64, s, c, 0};
+    if (d.min_p > 0.0f) {
+        const float f = (float)((double)m + d.T * log((double)d.min_p));
+        low = fmaxf(low, f - fabsf(f) * 2.4e-7f);  // NaN beside an infinite m: low stays
     }
     if (d.cuts) {
+#pragma unroll
+        for (int t = 0; t < kPer; t++) {
+            if (!(v[t] >= low)) continue;
+            int down;
+            const uint64_t w = draw_weight(unit, v[t], kCutBits, tab, down);
+            atomicAdd((unsigned long long *)&hist[down >> kBinShift], (unsigned long long)(w | 1ull << 50));
+        }
+        __syncthreads();
         const size_t at = (row * P + p) * kBins;
-        for (int b = tid; b < kBins; b += kDrawThreads) {
-            W.sum[at + b] = hsum[b];
-            W.cnt[at + b] = (uint16_t)hcnt[b];
+        for (int b = tid; b < kBins; b += kDrawThreads) W.hist[at + b] = hist[b];
+        if (tid == 0) *out = DrawPiece{m, 0, e, 0};
+    } else {
+        uint64_t s = 0;
+#pragma unroll
+        for (int t = 0; t < kPer; t++) {
+            if (!(v[t] >= low)) continue;
+            int down;
+            s += draw_weight(unit, v[t], kPlainBits, tab, down);
+        }
+        s = wave_sum(s);
+        if (lane == 0) ss[wave] = s;
+        __syncthreads();
+        if (tid == 0) {
+            s = 0;
+            for (int w = 0; w < 16; w++) s += ss[w];
+            *out = DrawPiece{m, 0, e, s};
         }
     }
 }
@@ -248,276 +272,23 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_scan(const void *__restri
 // those up to index `last`.
 struct DrawCut {
     uint32_t key, last;
+    __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
-__device__ __forceinline__ bool cut_keeps(const DrawCut &c, uint32_t key, uint32_t i) {
-    return key > c.key || (key == c.key && i <= c.last);
-}
 
 struct PickShared {
-    double tab[64];
+    double tab[kSteps];
     DrawPiece piece[kMaxPieces];
-    uint64_t kept[kMaxPieces];      // kept sums of the pieces
-    double sum[kBins];              // of the row's bins, below the row's octave
+    uint64_t kept[kMaxPieces];  // kept sums of the pieces, in their units
+    double sum[kBins];          // the row's bins, in the row's unit
     uint32_t cnt[kBins];
-    uint64_t sub_sum[kBins];        // of a key range's parts
+    uint64_t sub_sum[kBins];    // of a key range's parts
     uint32_t sub_cnt[kBins];
-    uint32_t list_key[kList], list_idx[kList];
+    uint32_t list_key[kList], list_idx[kList];  // tokens of one bin
     uint32_t list_n;
-    int list_bin;
-    int todo[kMaxPieces], ntodo;    // pieces that have tokens in the bin asked for
-    double red_d[16];
-    uint64_t red_u[16];
-    uint32_t red_i[16];
-    double pick_before;
-    uint32_t pick_at, pick_cnt;
-    uint32_t token;
-    float logit;
-};
-
-template <bool F16>
-struct Picker {
-    PickShared &S;
-    const void *logits;
-    size_t base, row;
-    int n, P;
-    bool aligned;
-    DrawRow d;
-    DrawWork W;
-    float m;
-    double e64;
-
-    __device__ bool inf() const { return m == INFINITY; }
-    // where bins of a piece start among the row's
-    __device__ int shift(int p) const {
-        const double s = (e64 - S.piece[p].e64) * 0.125;
-        return s < (double)kBins ? (int)s : kBins;
-    }
-    __device__ int bin_of(float l) const { return draw_bin(draw_q(l, d.c64, inf()), e64); }
-    // A weight with kBinBits bits below the octave that holds this bin's top:
-    // a bin can hold all 2^20 tokens of a row.
-    static constexpr int kBinBits = 40;
-    __device__ double bin_top64(int bin) const { return e64 - 64.0 * (bin >> 3); }
-    __device__ uint64_t weight_at(float l, double top64) const {
-        return draw_weight(l, d.c64, draw_q(l, d.c64, inf()), top64, inf(), S.tab) >> (kBits - kBinBits);
-    }
-
-    // fn(key, index, logit) for every token of a bin; from the list in LDS if it holds this bin
-    template <typename Fn>
-    __device__ void for_bin(int bin, Fn fn) {
-        if (S.list_bin == bin) {
-            for (uint32_t i = threadIdx.x; i < S.list_n; i += kDrawThreads)
-                fn(S.list_key[i], S.list_idx[i], lg_unkey(S.list_key[i]));
-            return;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) S.ntodo = 0;
-        __syncthreads();
-        if ((int)threadIdx.x < P) {
-            const int p = threadIdx.x, b = bin - shift(p);
-            // the row's last bin gathers what the pieces have from there on
-            if (S.piece[p].m > -INFINITY && (bin == kBins - 1 || (b >= 0 && W.cnt[(row * P + p) * kBins + b])))
-                S.todo[atomicAdd(&S.ntodo, 1)] = p;
-        }
-        __syncthreads();
-        constexpr int AT = 4;  // pieces in flight
-        for (int t = 0; t < S.ntodo; t += AT) {
-            float v[AT][kPer];
-#pragma unroll
-            for (int a = 0; a < AT; a++)
-                if (t + a < S.ntodo) piece_load<F16>(logits, base, S.todo[t + a] * kPiece, n, aligned, v[a]);
-#pragma unroll
-            for (int a = 0; a < AT; a++) {
-                if (t + a >= S.ntodo) break;
-                const int i0 = S.todo[t + a] * kPiece;
-#pragma unroll
-                for (int e = 0; e < kPer; e++) {
-                    const int i = i0 + piece_token<F16>(aligned, e);
-                    if (i < n && bin_of(v[a][e]) == bin) fn(lg_key(v[a][e]), (uint32_t)i, v[a][e]);
-                }
-            }
-        }
-    }
-
-    __device__ void gather(int bin) {
-        __syncthreads();
-        if (S.list_bin == bin || S.cnt[bin] > kList) return;
-        if (threadIdx.x == 0) S.list_n = 0;
-        __syncthreads();
-        for_bin(bin, [&](uint32_t key, uint32_t i, float) {
-            const uint32_t at = atomicAdd(&S.list_n, 1u);
-            if (at < kList) S.list_key[at] = key, S.list_idx[at] = i;
-        });
-        __syncthreads();
-        if (threadIdx.x == 0) S.list_bin = S.list_n <= kList ? bin : -1;
-        __syncthreads();
-    }
-
-    // The first bin at which the running count (by_count) or sum reaches the goal, with what goes before it.
-    __device__ int find_bin(bool by_count, double goal, double &before) {
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            const int lane = threadIdx.x;
-            double own[8], s = 0.0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                own[j] = by_count ? (double)S.cnt[8 * lane + j] : S.sum[8 * lane + j];
-                s += own[j];
-            }
-            double run = s;
-            for (int o = 1; o < 64; o <<= 1) {
-                const double v = __shfl_up(run, o);
-                if (lane >= o) run += v;
-            }
-            const uint64_t hit = __ballot(run >= goal && run > 0.0);
-            const uint64_t some = __ballot(s > 0.0);
-            const int at = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
-            if (lane == at) {
-                double b = run - s;  // at most a rounding off the lane below's run
-                int j = 0, last = 0;
-                double last_b = b;
-                for (; j < 8; j++) {
-                    if (own[j] > 0.0) last = j, last_b = b;
-                    if (own[j] > 0.0 && b + own[j] >= goal) break;
-                    b += own[j];
-                }
-                S.pick_at = 8 * lane + last;
-                S.pick_before = last_b;
-            }
-        }
-        __syncthreads();
-        before = S.pick_before;
-        return (int)S.pick_at;
-    }
-
-    // Within a bin: the token at which the goal is reached.  Keys are narrowed
-    // by 512 parts of their range until one key is left; its tokens weigh the
-    // same, so a division tells how many of them stay.  before and goal count
-    // tokens or, with weights, are integers below the bin's top.
-    __device__ DrawCut resolve(int bin, bool by_count, uint64_t goal, const DrawCut &lim, bool limited) {
-        const double top64 = bin_top64(bin);
-        uint32_t klo = 0xFFFFFFFFu, khi = 0;
-        gather(bin);
-        for_bin(bin, [&](uint32_t key, uint32_t i, float) {
-            if (limited && !cut_keeps(lim, key, i)) return;
-            klo = min(klo, key);
-            khi = max(khi, key);
-        });
-        for (int s = 32; s; s >>= 1) {
-            klo = min(klo, (uint32_t)__shfl_xor((int)klo, s));
-            khi = max(khi, (uint32_t)__shfl_xor((int)khi, s));
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) S.red_i[threadIdx.x >> 6] = klo, S.red_u[threadIdx.x >> 6] = khi;
-        __syncthreads();
-        for (int w = 0; w < 16; w++) klo = min(klo, S.red_i[w]), khi = max(khi, (uint32_t)S.red_u[w]);
-        uint64_t before = 0;
-        uint32_t ties = 0;
-        for (;;) {
-            int sh = 0;
-            while ((khi - klo) >> sh >= kBins) sh++;
-            __syncthreads();
-            for (int b = threadIdx.x; b < kBins; b += kDrawThreads) S.sub_sum[b] = 0, S.sub_cnt[b] = 0;
-            __syncthreads();
-            for_bin(bin, [&](uint32_t key, uint32_t i, float l) {
-                if (key < klo || key > khi || (limited && !cut_keeps(lim, key, i))) return;
-                const uint32_t b = (khi - key) >> sh;
-                atomicAdd(&S.sub_cnt[b], 1u);
-                if (!by_count) atomicAdd((unsigned long long *)&S.sub_sum[b], (unsigned long long)weight_at(l, top64));
-            });
-            __syncthreads();
-            if (threadIdx.x < 64) {
-                const int lane = threadIdx.x;
-                uint64_t own[8], s = 0;
-                uint32_t any = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    own[j] = by_count ? S.sub_cnt[8 * lane + j] : S.sub_sum[8 * lane + j];
-                    any |= S.sub_cnt[8 * lane + j];
-                    s += own[j];
-                }
-                uint64_t run = s;
-                for (int o = 1; o < 64; o <<= 1) {
-                    const uint64_t v = __shfl_up(run, o);
-                    if (lane >= o) run += v;
-                }
-                const uint64_t hit = __ballot(any && before + run >= goal);
-                const uint64_t some = __ballot(any != 0);
-                const int at = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
-                if (lane == at) {
-                    uint64_t b = before + run - s, last_b = b;
-                    int last = 0;
-                    for (int j = 0; j < 8; j++) {
-                        if (S.sub_cnt[8 * lane + j] == 0) continue;
-                        last = j, last_b = b;
-                        if (b + own[j] >= goal) break;
-                        b += own[j];
-                    }
-                    S.pick_at = 8 * lane + last;
-                    S.pick_cnt = S.sub_cnt[8 * lane + last];
-                    S.red_u[0] = last_b;
-                }
-            }
-            __syncthreads();
-            before = S.red_u[0];
-            ties = S.pick_cnt;
-            const uint32_t b = S.pick_at;
-            const uint32_t top = khi - (b << sh);
-            klo = sh == 0 ? top : max(klo, top - ((1u << sh) - 1u));
-            khi = top;
-            if (sh == 0) break;
-        }
-        uint64_t w = 1, left = goal > before ? goal - before : 0;
-        if (!by_count) w = weight_at(lg_unkey(klo), top64);
-        uint64_t c = w ? (left + w - 1) / w : 0;
-        c = c < 1 ? 1 : c;
-        DrawCut r{klo, 0xFFFFFFFFu};
-        if (limited && lim.key == klo) r.last = lim.last;
-        if (c < ties) r.last = nth_tie(bin, klo, (uint32_t)c);
-        return r;
-    }
-
-    // Index of the c-th token of a key that lies in this bin.
-    __device__ uint32_t nth_tie(int bin, uint32_t key, uint32_t c) {
-        uint32_t lo = 0, hi = (uint32_t)n - 1;  // the smallest index i with c ties up to it
-        while (lo < hi) {
-            const uint32_t step = (hi - lo) / kBins + 1;  // parts of the index range
-            __syncthreads();
-            for (int b = threadIdx.x; b < kBins; b += kDrawThreads) S.sub_cnt[b] = 0;
-            __syncthreads();
-            for_bin(bin, [&](uint32_t k, uint32_t i, float) {
-                if (k == key && i >= lo && i <= hi) atomicAdd(&S.sub_cnt[(i - lo) / step], 1u);
-            });
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                uint32_t b = 0, got = 0;
-                while (b < kBins - 1 && got + S.sub_cnt[b] < c) got += S.sub_cnt[b++];
-                S.pick_at = b;
-                S.pick_cnt = got;
-            }
-            __syncthreads();
-            c -= S.pick_cnt;
-            lo += S.pick_at * step;
-            hi = min(hi, lo + step - 1);
-        }
-        return lo;
-    }
-
-    // The kept part of a cut's own bin, in the row's units.
-    __device__ double bin_sum(int bin, const DrawCut &c) {
-        const double top64 = bin_top64(bin);
-        uint64_t s = 0;
-        for_bin(bin, [&](uint32_t key, uint32_t i, float l) {
-            if (cut_keeps(c, key, i)) s += weight_at(l, top64);
-        });
-        s = wave_sum(s);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) S.red_u[threadIdx.x >> 6] = s;
-        __syncthreads();
-        s = 0;
-        for (int w = 0; w < 16; w++) s += S.red_u[w];
-        __syncthreads();
-        return ldexp((double)s, kBits - kBinBits - (bin >> 3));
-    }
+    int todo[kMaxPieces], ntodo;  // pieces that have tokens in a bin
+    double before_d, red[16];
+    uint64_t before_u;
+    uint32_t at, ties, klo, khi;
 };
 
 template <bool F16>
@@ -527,180 +298,390 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_pick(const void *__restri
                                                             float *__restrict__ logp, DrawWork W) {
     __shared__ PickShared S;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t row = blockIdx.x;
-    Picker<F16> K{S, logits, row * n, row, n, P, aligned, draw_row(filter + 4 * row, n), W, -INFINITY, -kInfE};
-    const DrawRow &d = K.d;
+    const size_t row = blockIdx.x, base = row * n;
+    const DrawRow d = draw_row(filter + 4 * row, n);
+    const uint64_t *hist = W.hist + row * P * kBins;
+    float u = rnd[row];
     if (tid < P) S.piece[tid] = W.piece[row * P + tid];
-    if (tid >= kDrawThreads - 64) S.tab[tid & 63] = exp2((double)(tid & 63) / 64.0);
-    if (tid == 0) S.list_bin = -1;
+    if (!d.greedy) draw_table(S.tab);
     __syncthreads();
+    float m = -INFINITY;
+    double e = -kInfE;
     uint32_t first = 0xFFFFFFFFu;
-    for (int p = 0; p < P; p++)
-        if (S.piece[p].m > K.m) K.m = S.piece[p].m, first = S.piece[p].idx;
-    for (int p = 0; p < P; p++) K.e64 = fmax(K.e64, S.piece[p].e64);
-    if (K.m == -INFINITY || d.greedy) {
+    for (int p = 0; p < P; p++) {
+        if (S.piece[p].m > m) m = S.piece[p].m, first = S.piece[p].idx;
+        e = fmax(e, S.piece[p].e);
+    }
+    if (m == -INFINITY || d.greedy) {
         if (tid == 0) {
-            token[row] = K.m == -INFINITY ? 0xFFFFFFFFu : first;
-            if (logp) logp[row] = K.m == -INFINITY ? -INFINITY : 0.0f;
+            token[row] = m == -INFINITY ? 0xFFFFFFFFu : first;
+            if (logp) logp[row] = m == -INFINITY ? -INFINITY : 0.0f;
         }
         return;
     }
-    auto octaves = [&](int p) {  // of a piece's unit below the row's
-        return (int)fmin((K.e64 - S.piece[p].e64) * 0.015625, 4000.0);
-    };
+    // a piece's unit below the row's in octaves, and its first bin among the row's
+    auto octaves = [&](int p) { return (int)fmin((e - S.piece[p].e) * (1.0 / kSteps), 4000.0); };
+    auto shift = [&](int p) { return min(8 * octaves(p), kBins); };
+    const DrawUnit unit(d.c, e, m);
+    const float low = draw_low(m, d);
     DrawCut cut{0, 0xFFFFFFFFu};
-    int cbin = kBins;  // the bin of the cut
+    int cbin = kBins;  // the cut's bin; kBins: no cut
     if (d.cuts) {
         if (tid < kBins) {
             double s = 0.0;
             uint32_t c = 0;
-            for (int p = 0; p < P; p++) {
-                if (S.piece[p].m == -INFINITY) continue;
-                const int sh = K.shift(p);
-                const size_t at = (row * P + p) * kBins;
-                if (tid < sh || tid == kBins - 1) continue;
-                s += ldexp((double)W.sum[at + tid - sh], -octaves(p));
-                c += W.cnt[at + tid - sh];
+            for (int p0 = 0; p0 < P; p0 += 8) {
+                uint64_t h[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const int p = p0 + x, b = p < P && S.piece[p].m > -INFINITY ? tid - shift(p) : -1;
+                    h[x] = b >= 0 ? hist[p * kBins + b] : 0;
+                }
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    if (p0 + x >= P) break;
+                    s += ldexp((double)(h[x] & kSumMask), -octaves(p0 + x));
+                    c += (uint32_t)(h[x] >> 50);
+                }
             }
             S.sum[tid] = s;
             S.cnt[tid] = c;
-            c = wave_sum(c);
-            if (lane == 0) S.red_i[wave] = c;
         }
-        __syncthreads();
-        if (tid == 0) {  // the last bin: all the others; 63 octaves down, no weight is left
-            uint32_t c = 0;
-            for (int p = 0; p < P; p++) c += S.piece[p].cnt;
-            for (int w = 0; w < kBins / 64; w++) c -= S.red_i[w];
-            S.cnt[kBins - 1] = c;
-        }
-        __syncthreads();
-        double before;
         if (d.min_p > 0.0f) {  // the smallest float whose weight is at least min_p
-            const double lim = K.inf() ? INFINITY : (double)K.m + d.T * log((double)d.min_p);
+            const double lim = m == INFINITY ? INFINITY : (double)m + d.T * log((double)d.min_p);
             float f = (float)lim;
             if ((double)f < lim) f = lg_unkey(lg_key(f + 0.0f) + 1);
-            f = fminf(f + 0.0f, K.m);
-            if (f > -INFINITY) {
+            f = fminf(f + 0.0f, m);
+            if (f >= low) {
+                double r;
                 cut.key = lg_key(f);
-                cbin = K.bin_of(f);
+                cbin = (unit.sharp ? kSharpDown : -unit.steps(f, r)) >> kBinShift;
             }
         }
-        if (d.top_k) {
-            const int b = K.find_bin(true, (double)d.top_k, before);
-            if (b <= cbin && before + S.cnt[b] >= (double)d.top_k) {
-                const DrawCut c = K.resolve(b, true, d.top_k - (uint64_t)before, cut, false);
-                if (c.key >= cut.key) cut = c, cbin = b;
+        // the keys of a bin into S.klo .. S.khi: its borders in l, exactly, from the floats around them
+        auto bin_keys = [&](int bin) {
+            __syncthreads();
+            if (wave == 0) {
+                if (unit.sharp) {
+                    if (lane == 0) S.klo = S.khi = lg_key(m);
+                } else {
+                    uint32_t at[2];
+#pragma unroll
+                    for (int side = 0; side < 2; side++) {  // the first key of this bin, of the bin above
+                        const int steps = (bin + 1 - side) << kBinShift;
+                        float f = (float)((e - steps + 0.5) / d.c);
+                        f = f == f ? fminf(fmaxf(f, kLeast), -kLeast) : 0.0f;
+                        const uint32_t k0 = lg_key(f + 0.0f) - 32;
+                        const float l = lg_unkey(k0 + lane);
+                        double r;
+                        const uint64_t yes = __ballot(l > m || (l >= low && -unit.steps(l, r) < steps));
+                        at[side] = k0 + (yes ? __ffsll((long long)yes) - 1 : 64);
+                    }
+                    if (lane == 0) S.klo = at[0], S.khi = min(at[1] - 1, lg_key(m));
+                }
             }
-        }
-        if (d.top_p < 1.0f) {
-            double total;
-            if (cbin < kBins) {  // the cut's bin counts as far as it is kept
-                const double part = K.bin_sum(cbin, cut);
-                __syncthreads();
-                if (tid < kBins && tid >= cbin) S.sum[tid] = tid == cbin ? part : 0.0;
-                __syncthreads();
+            __syncthreads();
+        };
+        // fn(key, index, logit) for a bin's tokens with keys in [klo, khi], from
+        // the pieces that have any, AT pieces in flight
+        auto row_pass = [&](auto at_c, int bin, uint32_t klo, uint32_t khi, auto fn) {
+            constexpr int AT = decltype(at_c)::value;
+            __syncthreads();
+            if (tid == 0) S.ntodo = 0;
+            __syncthreads();
+            if (tid < P) {
+                const int b = bin - shift(tid);
+                if (S.piece[tid].m > -INFINITY && b >= 0 && hist[tid * kBins + b]) S.todo[atomicAdd(&S.ntodo, 1)] = tid;
             }
-            total = 0.0;
-            {
-                double s = tid < kBins ? S.sum[tid] : 0.0;
+            __syncthreads();
+            const float llo = lg_unkey(klo), lhi = lg_unkey(khi);
+            for (int t = 0; t < S.ntodo; t += AT) {
+                float v[AT][kPer];
+#pragma unroll
+                for (int a = 0; a < AT; a++)
+                    if (t + a < S.ntodo) piece_load<F16>(logits, base, S.todo[t + a] * kPiece, n, aligned, v[a]);
+#pragma unroll
+                for (int a = 0; a < AT; a++) {
+                    if (t + a >= S.ntodo) break;
+                    const int i0 = S.todo[t + a] * kPiece;
+#pragma unroll
+                    for (int x = 0; x < kPer; x++)
+                        if (v[a][x] >= llo && v[a][x] <= lhi) fn(lg_key(v[a][x]), (uint32_t)(i0 + piece_token<F16>(aligned, x)));
+                }
+            }
+        };
+        int listed = -1;  // the bin in the list, with its keys from list_lo to list_hi
+        uint32_t list_lo = 0, list_hi = 0;
+        auto holds = [&](int bin, uint32_t klo, uint32_t khi) { return listed == bin && klo >= list_lo && khi <= list_hi; };
+        auto bin_pass = [&](int bin, uint32_t klo, uint32_t khi, auto fn) {
+            if (holds(bin, klo, khi)) {
+                for (uint32_t i = tid; i < S.list_n; i += kDrawThreads) {
+                    const uint32_t k = S.list_key[i];
+                    if (k >= klo && k <= khi) fn(k, S.list_idx[i]);
+                }
+            } else {
+                row_pass(std::integral_constant<int, 1>{}, bin, klo, khi, fn);
+            }
+        };
+        // stage 0: top-k (min-p has set its key already); stage 1: top-p of what that leaves
+        for (int stage = 0; stage < 2; stage++) {
+            const bool by_count = stage == 0;
+            if (by_count ? d.top_k == 0 && cbin == kBins : d.top_p >= 1.0f) continue;
+            if (!by_count || d.top_k) {
+                double goal = d.top_k;
+                if (!by_count) {
+                    double s = 0.0;
+                    if (cbin < kBins)
+                        for (int p = tid; p < P; p += kDrawThreads) s += ldexp((double)S.kept[p], -octaves(p));
+                    else if (tid < kBins)
+                        s = S.sum[tid];
+                    s = wave_sum(s);
+                    __syncthreads();
+                    if (lane == 0) S.red[wave] = s;
+                    __syncthreads();
+                    goal = 0.0;
+                    for (int w = 0; w < 16; w++) goal += S.red[w];
+                    goal *= (double)d.top_p;
+                }
+                // the first bin at which the running count or sum reaches the goal
+                __syncthreads();
+                if (wave == 0) {
+                    double own[8], s = 0.0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int b = 8 * lane + j;
+                        own[j] = by_count ? (double)S.cnt[b] : b < cbin ? S.sum[b] : 0.0;
+                        s += own[j];
+                    }
+                    double run = s;
+                    for (int o = 1; o < 64; o <<= 1) {
+                        const double x = __shfl_up(run, o);
+                        if (lane >= o) run += x;
+                    }
+                    const uint64_t hit = __ballot(run >= goal && run > 0.0);
+                    if (hit == 0 && lane == 63) S.at = kBins, S.before_d = run;
+                    if (hit && lane == __ffsll((long long)hit) - 1) {
+                        double b = run - s, last_b = b;
+                        int last = 0;
+                        bool done = false;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            if (!done && own[j] > 0.0) last = j, last_b = b;
+                            done = done || (own[j] > 0.0 && b + own[j] >= goal);
+                            b += own[j];
+                        }
+                        S.at = 8 * lane + last;
+                        S.before_d = last_b;
+                    }
+                }
+                __syncthreads();
+                int bin = S.at;
+                const double before_d = S.before_d;
+                if (!by_count && bin == kBins) bin = cbin;  // not above the cut's bin: in it
+                // a count that ends below the cut, or among tokens without weight, cuts nothing
+                if (bin <= cbin && bin < kDeepBin) {
+                    const bool limited = bin == cbin;
+                    const DrawCut lim = cut;
+                    bin_keys(bin);
+                    const uint32_t klo0 = limited ? max(S.klo, lim.key) : S.klo;
+                    uint32_t klo = klo0, khi = max(S.khi, klo0);
+                    // the goal inside the bin: a count, or weights kInBits below the octave that holds the bin's top
+                    const double left = fmax(goal - before_d, 0.0);
+                    const uint64_t want = by_count ? (uint64_t)left : (uint64_t)ceil(ldexp(left, (bin >> 3) + kInBits - kCutBits));
+                    const DrawUnit in_unit(d.c, e - (double)kSteps * (bin >> 3), m);
+                    uint64_t before = 0;
+                    uint32_t cnt = S.cnt[bin], ties = 0;
+                    for (;;) {  // keys are narrowed by 512 parts of their range until one is left
+                        if (cnt <= kList && !holds(bin, klo, khi)) {
+                            __syncthreads();
+                            if (tid == 0) S.list_n = 0;
+                            row_pass(std::integral_constant<int, 4>{}, bin, klo, khi, [&](uint32_t k, uint32_t i) {
+                                const uint32_t x = atomicAdd(&S.list_n, 1u);
+                                if (x < kList) S.list_key[x] = k, S.list_idx[x] = i;
+                            });
+                            __syncthreads();
+                            listed = S.list_n <= kList ? bin : -1;
+                            list_lo = klo;
+                            list_hi = khi;
+                        }
+                        int sh = 0;
+                        while ((khi - klo) >> sh >= kBins) sh++;
+                        __syncthreads();
+                        if (tid < kBins) S.sub_sum[tid] = 0, S.sub_cnt[tid] = 0;
+                        __syncthreads();
+                        bin_pass(bin, klo, khi, [&](uint32_t k, uint32_t i) {
+                            if (limited && !lim.keeps(k, i)) return;
+                            const uint32_t b = (khi - k) >> sh;
+                            int down;
+                            atomicAdd(&S.sub_cnt[b], 1u);
+                            if (!by_count)
+                                atomicAdd((unsigned long long *)&S.sub_sum[b], (unsigned long long)draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down));
+                        });
+                        __syncthreads();
+                        if (wave == 0) {
+                            uint64_t own[8], s = 0;
+                            uint32_t c[8], some = 0;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                c[j] = S.sub_cnt[8 * lane + j];
+                                own[j] = by_count ? c[j] : S.sub_sum[8 * lane + j];
+                                some |= c[j];
+                                s += own[j];
+                            }
+                            uint64_t run = s;
+                            for (int o = 1; o < 64; o <<= 1) {
+                                const uint64_t x = __shfl_up(run, o);
+                                if (lane >= o) run += x;
+                            }
+                            if (lane == 0) S.at = 0, S.ties = 0, S.before_u = before;  // stands if the range is empty
+                            const uint64_t any = __ballot(some != 0), hit = __ballot(some != 0 && before + run >= want);
+                            if (lane == (hit ? __ffsll((long long)hit) : 64 - __clzll((long long)any)) - 1) {
+                                uint64_t b = before + run - s, last_b = b;
+                                uint32_t last = 0, last_c = 0;
+                                bool done = false;
+#pragma unroll
+                                for (int j = 0; j < 8; j++) {
+                                    if (!done && c[j]) last = j, last_c = c[j], last_b = b;
+                                    done = done || (c[j] && b + own[j] >= want);
+                                    b += own[j];
+                                }
+                                S.at = 8 * lane + last;
+                                S.ties = last_c;
+                                S.before_u = last_b;
+                            }
+                        }
+                        __syncthreads();
+                        before = S.before_u;
+                        cnt = ties = S.ties;
+                        khi -= S.at << sh;
+                        if (sh == 0) break;
+                        klo = max(klo, khi - ((1u << sh) - 1u));
+                    }
+                    // one key is left; its tokens weigh the same, so a division tells how many stay
+                    int down;
+                    const uint64_t w = by_count ? 1 : draw_weight(in_unit, lg_unkey(khi), kInBits, S.tab, down);
+                    uint32_t c = want > before && w ? (uint32_t)min((unsigned long long)((want - before + w - 1) / w), (unsigned long long)n) : 1;
+                    cut = DrawCut{khi, limited && lim.key == khi ? lim.last : 0xFFFFFFFFu};
+                    cbin = bin;
+                    if (c < ties) {  // the index of the c-th token of this key, by 512 parts of the index range
+                        uint32_t lo = 0, hi = (uint32_t)n - 1;
+                        while (lo < hi) {
+                            const uint32_t step = (hi - lo) / kBins + 1;
+                            __syncthreads();
+                            if (tid < kBins) S.sub_cnt[tid] = 0;
+                            __syncthreads();
+                            bin_pass(bin, khi, khi, [&](uint32_t, uint32_t i) {
+                                if (i >= lo && i <= hi) atomicAdd(&S.sub_cnt[(i - lo) / step], 1u);
+                            });
+                            __syncthreads();
+                            if (tid == 0) {
+                                uint32_t b = 0, got = 0;
+                                while (b < kBins - 1 && got + S.sub_cnt[b] < c) got += S.sub_cnt[b++];
+                                S.at = b;
+                                S.ties = got;
+                            }
+                            __syncthreads();
+                            c -= S.ties;
+                            lo += S.at * step;
+                            hi = min(hi, lo + step - 1);
+                        }
+                        cut.last = lo;
+                    }
+                }
+            }
+            if (cbin == kBins) continue;
+            // kept sums of the pieces: whole bins, and the cut's own bin token by token
+            bin_keys(cbin);
+            for (int p = wave; p < P; p += 16) {
+                uint64_t s = 0;
+                const int top = S.piece[p].m > -INFINITY ? cbin - shift(p) : 0;
+#pragma unroll
+                for (int x = 0; x < kBins; x += 64) s += x + lane < top ? hist[p * kBins + x + lane] & kSumMask : 0;
                 s = wave_sum(s);
-                if (lane == 0) S.red_d[wave] = s;
-                __syncthreads();
-                for (int w = 0; w < kBins / 64; w++) total += S.red_d[w];
+                if (lane == 0) S.kept[p] = s;
             }
-            const double goal = (double)d.top_p * total;
-            const int b = K.find_bin(false, goal, before);
-            const double left = fmax(goal - before, 0.0);
-            const bool lim = b == cbin;
-            cut = K.resolve(b, false, (uint64_t)ceil(ldexp(left, (b >> 3) + K.kBinBits - kBits)), cut, lim);
-            cbin = b;
+            const uint32_t top_key = S.khi;
+            __syncthreads();
+            bin_pass(cbin, cut.key, top_key, [&](uint32_t k, uint32_t i) {
+                if (!cut.keeps(k, i)) return;
+                const int p = i / kPiece;
+                const DrawUnit pu(d.c, S.piece[p].e, S.piece[p].m);
+                int down;
+                atomicAdd((unsigned long long *)&S.kept[p], (unsigned long long)draw_weight(pu, lg_unkey(k), kCutBits, S.tab, down));
+            });
+            __syncthreads();
         }
     }
-    // kept sums of the pieces
-    if (cbin < kBins) {
-        K.gather(cbin);
+    // Where no cut was found (all tokens stay) a row with cuts has its sums in the bins.
+    const int bits = d.cuts ? kCutBits : kPlainBits;
+    if (cbin == kBins) {
         for (int p = wave; p < P; p += 16) {
-            uint64_t s = 0;
-            if (S.piece[p].m > -INFINITY) {
-                const int sh = K.shift(p), top = min(kBins, cbin - sh);
-                for (int b = lane; b < top; b += 64) s += W.sum[(row * P + p) * kBins + b];
+            uint64_t s = S.piece[p].sum;
+            if (d.cuts) {
+                s = 0;
+                if (S.piece[p].m > -INFINITY)
+                    for (int x = lane; x < kBins; x += 64) s += hist[p * kBins + x] & kSumMask;
+                s = wave_sum(s);
             }
-            s = wave_sum(s);
             if (lane == 0) S.kept[p] = s;
         }
         __syncthreads();
-        K.for_bin(cbin, [&](uint32_t key, uint32_t i, float l) {
-            if (!cut_keeps(cut, key, i)) return;
-            const int p = i / kPiece;
-            const uint64_t w = draw_weight(l, d.c64, draw_q(l, d.c64, S.piece[p].m == INFINITY), S.piece[p].e64, S.piece[p].m == INFINITY, S.tab);
-            atomicAdd((unsigned long long *)&S.kept[p], (unsigned long long)w);
-        });
-    } else if (tid < P) {
-        S.kept[tid] = S.piece[tid].sum;
     }
-    __syncthreads();
     // the draw's piece
     double total = 0.0;
     for (int p = 0; p < P; p++) total += ldexp((double)S.kept[p], -octaves(p));
-    float u = rnd[row];
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     const double target = (double)u * total;
     double run = 0.0, at = 0.0;
     int piece = 0;
     for (int p = 0; p < P; p++) {
-        const double s = ldexp((double)S.kept[p], -octaves(p));
-        if (S.kept[p]) piece = p, at = run;
-        if (S.kept[p] && run + s > target) break;
-        run += s;
+        if (S.kept[p] == 0) continue;
+        piece = p;
+        at = run;
+        run += ldexp((double)S.kept[p], -octaves(p));
+        if (run > target) break;
     }
     // its token: lanes hold tokens of the piece in index order
-    const float pm = S.piece[piece].m;
-    const bool pinf = pm == INFINITY;
-    const double pe = S.piece[piece].e64;
+    const DrawUnit pu(d.c, S.piece[piece].e, S.piece[piece].m);
+    const float plow = draw_low(S.piece[piece].m, d);
     uint64_t goal = (uint64_t)fmax(ldexp(target - at, octaves(piece)), 0.0);
     if (goal >= S.kept[piece]) goal = S.kept[piece] - 1;
     float v[kPer];
     uint64_t w[kPer], mine = 0;
     const int i0 = piece * kPiece + tid * kPer;
 #pragma unroll
-    for (int e = 0; e < kPer; e++) {
-        v[e] = i0 + e < n ? lg_value<F16>(logits, K.base + i0 + e) : -INFINITY;
-        const bool keep = v[e] > -INFINITY && cut_keeps(cut, lg_key(v[e]), i0 + e);
-        w[e] = keep ? draw_weight(v[e], d.c64, draw_q(v[e], d.c64, pinf), pe, pinf, S.tab) : 0;
-        mine += w[e];
+    for (int x = 0; x < kPer; x++) v[x] = i0 + x < n ? lg_value<F16>(logits, base + i0 + x) : -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kPer; x++) {
+        int down;
+        w[x] = 0;
+        if (v[x] >= plow && cut.keeps(lg_key(v[x]), i0 + x)) w[x] = draw_weight(pu, v[x], bits, S.tab, down);
+        mine += w[x];
     }
     uint64_t pre = mine;
     for (int s = 1; s < 64; s <<= 1) {
         const uint64_t o = __shfl_up(pre, s);
         if (lane >= s) pre += o;
     }
-    __syncthreads();
-    if (lane == 63) S.red_u[wave] = pre;
+    uint64_t *wave_total = S.sub_sum;
+    if (lane == 63) wave_total[wave] = pre;
     __syncthreads();
     uint64_t b = pre - mine;
-    for (int x = 0; x < wave; x++) b += S.red_u[x];
+    for (int x = 0; x < wave; x++) b += wave_total[x];
     if (goal >= b && goal < b + mine) {
-        int hit = 0;
-        for (int e = 0; e < kPer; e++) {
-            if (goal < b + w[e]) {
-                hit = e;
-                break;
-            }
-            b += w[e];
-        }
-        float l = v[0];
+        int hit = -1;
+        float l = 0.0f;
 #pragma unroll
-        for (int e = 1; e < kPer; e++) l = hit == e ? v[e] : l;
+        for (int x = 0; x < kPer; x++) {
+            b += w[x];
+            if (hit < 0 && goal < b) hit = x, l = v[x];
+        }
         token[row] = i0 + hit;
-        if (logp) {  // in units of the row's octave: total 2^-kBits 2^E
-            const double z = l == K.m ? 0.0 : ((double)l - (double)K.m) / d.T;
-            double me = -1.0;  // the maximum's octaves below E, as draw_weight takes them
-            if (!K.inf()) {
-                const double q = draw_q(K.m, d.c64, false);
-                me = (q - K.e64 + draw_frac(K.m, d.c64, q)) / 64.0;
-            }
-            logp[row] = (float)(z - (log(ldexp(total, -kBits)) - me * 0.69314718055994530942));
+        if (logp) {  // the sum is total 2^(E - bits); the maximum lies `below` octaves under E
+            double r = 0.0, below = 1.0;
+            if (!unit.sharp) below = -(unit.steps(m, r) + 0.0) / kSteps, below -= r / kSteps;
+            const double z = l == m ? 0.0 : ((double)l - (double)m) / d.T;
+            logp[row] = (float)(z - (log(ldexp(total, -bits)) + below * 0.69314718055994530942));
         }
     }
 }
@@ -844,7 +825,7 @@ static int logprob_pieces(uint64_t n, uint64_t rows) {
 
 // ------------------------------------------------------------- launchers
 uint64_t logits_work_words(uint64_t n, uint64_t rows) {
-    const uint64_t draw = rows * draw_pieces(n) * (sizeof(DrawPiece) + kBins * 10) / 4;
+    const uint64_t draw = rows * draw_pieces(n) * (sizeof(DrawPiece) + kBins * 8) / 4;
     const uint64_t lp = rows * logprob_pieces(n, rows) * sizeof(LpPart) / 4;
     return std::max(draw, lp);
 }
@@ -861,9 +842,8 @@ int launch_draw(rsv_ctx *ctx, const void *logits, int f16, uint32_t *token, uint
                 const float *rnd, float *logp, float *work, uint64_t rows) {
     const int P = draw_pieces(n);
     DrawWork W;
-    W.sum = (uint64_t *)work;
-    W.piece = (DrawPiece *)(W.sum + rows * P * kBins);
-    W.cnt = (uint16_t *)(W.piece + rows * P);
+    W.hist = (uint64_t *)work;
+    W.piece = (DrawPiece *)(W.hist + rows * P * kBins);
     const bool aligned = n * (f16 ? 2 : 4) % 16 == 0;
     if (f16)
         draw_launch<true>(ctx, logits, (int)n, P, aligned, filter, rnd, token, logp, W, rows);

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "k_dpp.h"
 #include "rsv_common.h"
 
 namespace rsv {
@@ -15,6 +16,13 @@ __device__ __forceinline__ float lg_clean(float l) { return l == l ? l + 0.0f : 
 template <bool F16>
 __device__ __forceinline__ float lg_value(const void *p, size_t i) {
     return lg_clean(F16 ? (float)((const _Float16 *)p)[i] : ((const float *)p)[i]);
+}
+// One of 16 bytes' logits as it is.
+template <bool F16>
+__device__ __forceinline__ float raw_value(const uint4 &q, int x) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[x >> 1] >> (16 * (x & 1))));
+    else return __uint_as_float(w[x]);
 }
 // Order-preserving bits: larger logit, larger key.
 __device__ __forceinline__ uint32_t lg_key(float l) {
@@ -64,7 +72,8 @@ __device__ __forceinline__ void lg_unpack(uint4 q, float (&v)[F16 ? 8 : 4]) {
 // stand in no bin.  Rows that are only settled by their maximum (+inf, or
 // |l c| past 2^50, where different logits are 36 T apart) are `sharp`: tokens
 // at the maximum weigh 2^(bits - 1), the others nothing.
-constexpr int kPiece = 8192, kDrawThreads = 1024, kPer = kPiece / kDrawThreads;
+constexpr int kPiece = 8192, kGroup = 1024, kGroups = kPiece / kGroup;
+constexpr int kScanThreads = 512, kPickThreads = 256;
 constexpr int kBins = 512, kSteps = 1024, kBinShift = 7, kMaxPieces = (int)(kLogitsMaxN / kPiece);
 constexpr int kSharpDown = kSteps - 1;  // a sharp maximum stands in its first octave's last bin
 constexpr int kDeepBin = 50 * 8;  // from here on weights vanish beside the maximum's
@@ -72,13 +81,13 @@ constexpr int kPlainBits = 48;    // weights of a row without cuts
 constexpr int kCutBits = 37;      // with cuts: a bin packs its sum (8192 2^37 = 2^50) and above it its count
 constexpr int kInBits = 40;       // inside a bin, below the bin's octave: up to 2^20 tokens
 constexpr uint64_t kSumMask = ((uint64_t)1 << 50) - 1;
-constexpr int kList = 4096;       // a bin's tokens held in LDS
+constexpr int kList = 4096, kListRoom = kList + 8;  // a bin's tokens held in LDS; half a piece and a vector
 
 struct DrawPiece {
     float m;        // largest logit (-inf: nothing to draw)
     uint32_t idx;   // its lowest token (greedy rows)
     double e;       // 1024 E
-    uint64_t sum;   // plain rows
+    uint64_t sum, group[kGroups];  // of the piece and of each 1024 tokens (plain rows)
 };
 struct DrawWork {
     DrawPiece *piece;   // [rows, P]
@@ -149,83 +158,155 @@ __device__ __forceinline__ uint64_t draw_weight(const DrawUnit &u, float l, int 
     down = -k;
     return draw_value(k, r, bits, tab);
 }
-__device__ __forceinline__ void draw_table(double *tab) {
-    for (int i = threadIdx.x; i < kSteps; i += kDrawThreads) tab[i] = exp2((double)i / kSteps);
-}
-
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
-// The tokens of a piece that a lane holds, kPer of them, those past the row's
-// end as -inf.  `aligned`: rows start at 16-byte borders.
-template <bool F16>
-__device__ __forceinline__ int piece_token(bool aligned, int e) {
-    constexpr int V = F16 ? 8 : 4;
-    return aligned ? ((int)threadIdx.x + kDrawThreads * (e / V)) * V + e % V : (int)threadIdx.x + kDrawThreads * e;
-}
-template <bool F16>
-__device__ __forceinline__ void piece_load(const void *logits, size_t base, int i0, int n, bool aligned, float (&v)[kPer]) {
-    constexpr int V = F16 ? 8 : 4;
-    if (aligned && i0 + kPiece <= n) {
-#pragma unroll
-        for (int b = 0; b < kPer / V; b++) {
-            float w[V];
-            const size_t at = base + i0 + (threadIdx.x + kDrawThreads * b) * V;
-            lg_unpack<F16>(*(const uint4 *)((const char *)logits + at * (F16 ? 2 : 4)), w);
-#pragma unroll
-            for (int e = 0; e < V; e++) v[b * V + e] = w[e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < kPer; e++) {
-            const int i = i0 + piece_token<F16>(aligned, e);
-            v[e] = i < n ? lg_value<F16>(logits, base + i) : -INFINITY;
+// 2^(i / 1024), made by the compiler: the series of exp, smallest terms first.
+struct DrawTable {
+    double v[kSteps];
+    constexpr DrawTable() : v() {
+        for (int i = 0; i < kSteps; i++) {
+            const double x = 0.69314718055994530942 * i / kSteps;
+            double t[24] = {1.0}, sum = 0.0;
+            for (int k = 1; k < 24; k++) t[k] = t[k - 1] * x / k;
+            for (int k = 23; k >= 0; k--) sum += t[k];
+            v[i] = sum;
         }
     }
+};
+__device__ const DrawTable kDrawTable{};
+template <int NT>
+__device__ __forceinline__ void draw_table(double *tab) {
+#pragma unroll
+    for (int i = 0; i < kSteps / 2; i += NT)
+        if (kSteps / 2 % NT == 0 || i + (int)threadIdx.x < kSteps / 2) ((double2 *)tab)[i + threadIdx.x] = ((const double2 *)kDrawTable.v)[i + threadIdx.x];
 }
 
+// Sums over a wave by row shifts and broadcasts: the inclusive scan, whose last
+// lane holds the sum.
+template <int CTRL, int RM, typename T>
+__device__ __forceinline__ T dpp64(T v) {
+    static_assert(sizeof(T) == 8);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, RM, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, RM, 0xF, false);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp64<0x111, 0xF>(v);
+    v += dpp64<0x112, 0xF>(v);
+    v += dpp64<0x114, 0xF>(v);
+    v += dpp64<0x118, 0xF>(v);
+    v += dpp64<0x142, 0xA>(v);
+    v += dpp64<0x143, 0xC>(v);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T lane_of(T v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+}
+
+// A piece's tokens over NT threads: thread t has the 16-byte vectors t, t + NT,
+// ... from the border at or before the piece's first token on, and one more
+// where the row does not start at a border; tokens that are not the piece's
+// are -inf.  Vectors stay inside the tensor's memory, whose end is padded.
+template <bool F16, int NT>
+struct PieceView {
+    static constexpr int V = F16 ? 8 : 4, NV = kPiece / NT / V + 1, N = NV * V;
+    const uint4 *q;
+    int first, off, len;  // token of the border, piece's first token behind it, its tokens
+    __device__ __forceinline__ PieceView(const void *logits, size_t base, int p, int n) {
+        const size_t at = base + (size_t)p * kPiece;
+        off = (int)(at % V);
+        first = p * kPiece - off;
+        len = min(kPiece, n - p * kPiece);
+        q = (const uint4 *)((const char *)logits + (at - off) * (F16 ? 2 : 4));
+    }
+    __device__ __forceinline__ int token(int x) const { return first + ((int)threadIdx.x + NT * (x / V)) * V + x % V; }
+    __device__ __forceinline__ void load(uint4 (&r)[NV]) const {
+#pragma unroll
+        for (int b = 0; b < NV; b++) {
+            const int vec = (int)threadIdx.x + NT * b;
+            if (vec * V < len + off) r[b] = q[vec];
+        }
+    }
+    // sets what is not the piece's to -inf
+    __device__ __forceinline__ void edges(uint4 (&r)[NV]) const {
+#pragma unroll
+        for (int b = 0; b < NV; b++) {
+            const int i = ((int)threadIdx.x + NT * b) * V;
+            if (i >= off && i + V <= len + off) continue;
+            uint32_t w[4] = {r[b].x, r[b].y, r[b].z, r[b].w};
+#pragma unroll
+            for (int x = 0; x < V; x++) {
+                if (i + x >= off && i + x < len + off) continue;
+                if constexpr (F16)
+                    w[x >> 1] = x & 1 ? (w[x >> 1] & 0xFFFFu) | 0xFC000000u : (w[x >> 1] & 0xFFFF0000u) | 0xFC00u;
+                else
+                    w[x] = 0xFF800000u;
+            }
+            r[b] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    __device__ __forceinline__ void values(uint4 (&r)[NV], float (&v)[N]) const {
+        edges(r);
+#pragma unroll
+        for (int b = 0; b < NV; b++) {
+            float w[V];
+            lg_unpack<F16>(r[b], w);
+#pragma unroll
+            for (int x = 0; x < V; x++) v[b * V + x] = w[x];
+        }
+    }
+};
+
 template <bool F16>
-__global__ __launch_bounds__(kDrawThreads) void k_draw_scan(const void *__restrict__ logits, int n, int P, bool aligned,
+__global__ __launch_bounds__(kScanThreads) void k_draw_scan(const void *__restrict__ logits, int n, int P,
                                                             const float *__restrict__ filter, DrawWork W) {
+    constexpr int NT = kScanThreads, NW = NT / 64;
     __shared__ double tab[kSteps];
     __shared__ uint64_t hist[kBins];
-    __shared__ uint64_t ss[16];
-    __shared__ float sm[16];
-    __shared__ uint32_t si[16];
+    __shared__ uint64_t group[kGroups];
+    __shared__ float sm[NW];
+    __shared__ uint32_t si[NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t row = blockIdx.x / P;
-    const int p = blockIdx.x % P, i0 = p * kPiece;
-    float v[kPer];
-    piece_load<F16>(logits, row * n, i0, n, aligned, v);
+    const int p = blockIdx.x % P;
+    using View = PieceView<F16, NT>;
+    const View view(logits, row * n, p, n);
+    uint4 raw[View::NV];
+    view.load(raw);
     const DrawRow d = draw_row(filter + 4 * row, n);
-    if (!d.greedy) draw_table(tab);
+    if (!d.greedy) draw_table<NT>(tab);
     if (d.cuts)
-        for (int b = tid; b < kBins; b += kDrawThreads) hist[b] = 0;
+        for (int b = tid; b < kBins; b += NT) hist[b] = 0;
+    if (tid < kGroups) group[tid] = 0;
+    float v[View::N];
+    view.values(raw, v);
     float m = v[0];
 #pragma unroll
-    for (int e = 1; e < kPer; e++) m = fmaxf(m, v[e]);
-    for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-    if (lane == 0) sm[wave] = m;
+    for (int x = 1; x < View::N; x++) m = fmaxf(m, v[x]);
+    m = wave_max_last(m);
+    if (lane == 63) sm[wave] = m;
     __syncthreads();
-    for (int w = 0; w < 16; w++) m = fmaxf(m, sm[w]);
+    m = sm[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) m = fmaxf(m, sm[w]);
     DrawPiece *out = W.piece + row * P + p;
     if (d.greedy) {
         uint32_t idx = 0xFFFFFFFFu;
 #pragma unroll
-        for (int e = kPer - 1; e >= 0; e--)
-            if (v[e] == m) idx = i0 + piece_token<F16>(aligned, e);
+        for (int x = View::N - 1; x >= 0; x--)
+            if (v[x] == m) idx = min(idx, (uint32_t)view.token(x));  // where all are -inf the draw does not look
         for (int s = 32; s; s >>= 1) idx = min(idx, (uint32_t)__shfl_xor((int)idx, s));
         if (lane == 0) si[wave] = idx;
         __syncthreads();
-        for (int w = 0; w < 16; w++) idx = min(idx, si[w]);
-        if (tid == 0) *out = DrawPiece{m, idx, 0.0, 0};
+        for (int w = 0; w < NW; w++) idx = min(idx, si[w]);
+        if (tid == 0) out->m = m, out->idx = idx, out->e = 0.0;
         return;
     }
     if (m == -INFINITY) {
-        if (tid == 0) *out = DrawPiece{m, 0, -kInfE, 0};
+        if (tid == 0) out->m = m, out->e = -kInfE, out->sum = 0;
         return;
     }
     const double e = draw_e(m, d.c);
@@ -238,31 +319,36 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_scan(const void *__restri
     }
     if (d.cuts) {
 #pragma unroll
-        for (int t = 0; t < kPer; t++) {
-            if (!(v[t] >= low)) continue;
+        for (int x = 0; x < View::N; x++) {
+            if (!(v[x] >= low)) continue;
             int down;
-            const uint64_t w = draw_weight(unit, v[t], kCutBits, tab, down);
+            const uint64_t w = draw_weight(unit, v[x], kCutBits, tab, down);
             atomicAdd((unsigned long long *)&hist[down >> kBinShift], (unsigned long long)(w | 1ull << 50));
         }
         __syncthreads();
         const size_t at = (row * P + p) * kBins;
-        for (int b = tid; b < kBins; b += kDrawThreads) W.hist[at + b] = hist[b];
-        if (tid == 0) *out = DrawPiece{m, 0, e, 0};
+        for (int b = tid; b < kBins; b += NT) W.hist[at + b] = hist[b];
+        if (tid == 0) out->m = m, out->e = e;
     } else {
-        uint64_t s = 0;
+        // a wave's vectors lie in one group, if the row starts at a border
 #pragma unroll
-        for (int t = 0; t < kPer; t++) {
-            if (!(v[t] >= low)) continue;
-            int down;
-            s += draw_weight(unit, v[t], kPlainBits, tab, down);
+        for (int x0 = 0; x0 < View::N; x0 += View::V) {
+            uint64_t s = 0;
+#pragma unroll
+            for (int x = x0; x < x0 + View::V; x++) {
+                int down;
+                if (v[x] >= low) s += draw_weight(unit, v[x], kPlainBits, tab, down);
+            }
+            s = wave_scan(s);
+            const int g = (wave * 64 + NT * (x0 / View::V)) * View::V / kGroup;
+            if (lane == 63 && s) atomicAdd((unsigned long long *)&group[min(g, kGroups - 1)], (unsigned long long)s);
         }
-        s = wave_sum(s);
-        if (lane == 0) ss[wave] = s;
         __syncthreads();
+        if (tid < kGroups) out->group[tid] = group[tid];
         if (tid == 0) {
-            s = 0;
-            for (int w = 0; w < 16; w++) s += ss[w];
-            *out = DrawPiece{m, 0, e, s};
+            uint64_t s = 0;
+            for (int g = 0; g < kGroups; g++) s += group[g];
+            out->m = m, out->e = e, out->sum = s;
         }
     }
 }
@@ -275,42 +361,113 @@ struct DrawCut {
     __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
 
-struct PickShared {
+constexpr int kFew = 8;  // pieces whose histograms and tokens are held at once (n <= 65536)
+// Eight bins a lane, with a gap behind each eight against bank conflicts.
+__device__ __forceinline__ int bin_at(int b) { return b + (b >> 3); }
+constexpr int kBinRoom = kBins + kBins / 8;
+
+// A piece without its groups.
+struct DrawHead {
+    float m;
+    uint32_t idx;
+    double e;
+    uint64_t sum;
+};
+struct __align__(16) PickShared {
     double tab[kSteps];
-    DrawPiece piece[kMaxPieces];
-    uint64_t kept[kMaxPieces];  // kept sums of the pieces, in their units
-    double sum[kBins];          // the row's bins, in the row's unit
-    uint32_t cnt[kBins];
-    uint64_t sub_sum[kBins];    // of a key range's parts
-    uint32_t sub_cnt[kBins];
-    uint32_t list_key[kList], list_idx[kList];  // tokens of one bin
+    uint64_t hist[kFew * kBins];   // of the row's pieces, where they are few
+    DrawHead piece[kMaxPieces];
+    double scale[kMaxPieces];      // a piece's unit in the row's
+    int shift[kMaxPieces];         // its first bin among the row's
+    uint64_t kept[kMaxPieces];     // its kept sum, in its unit
+    double sum[kBinRoom];          // the row's bins, in the row's unit
+    uint32_t cnt[kBinRoom];
+    uint64_t sub_sum[kBinRoom];    // of a key range's parts
+    uint32_t sub_cnt[kBinRoom];
+    union {
+        struct {
+            uint32_t list_key[kListRoom], list_idx[kListRoom];  // tokens of one bin
+        };
+        float tok[kPiece + kPiece / 8 + 16];  // at last the draw's piece
+    };
     uint32_t list_n;
-    int todo[kMaxPieces], ntodo;  // pieces that have tokens in a bin
-    double before_d, red[16];
-    uint64_t before_u;
-    uint32_t at, ties, klo, khi;
+    int todo[kMaxPieces], ntodo;   // pieces that have tokens in a bin
+    double before_d;
+    uint64_t before_u, wave_total[kPickThreads / 64];
+    uint32_t at, ties;
 };
 
+// In wave 0: the first of 512 parts (eight a lane) at which `before` and what
+// has gone by reach the goal, or the last part that holds anything.
+template <typename T>
+__device__ __forceinline__ int first_part(const T (&own)[8], const bool (&some)[8], T before, T goal, T &gone) {
+    T s = own[0];
+    bool any = some[0];
+#pragma unroll
+    for (int j = 1; j < 8; j++) s += own[j], any = any || some[j];
+    const T run = before + wave_scan(s);
+    const uint64_t anys = __ballot(any), hits = __ballot(any && run >= goal);
+    if (anys == 0) return -1;
+    const int lane = hits ? __ffsll((long long)hits) - 1 : 63 - __clzll((long long)anys);
+    T b = run - s;
+    int last = 0;
+    bool done = false;
+    gone = b;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        if (!done && some[j]) last = j, gone = b;
+        done = done || (some[j] && b + own[j] >= goal);
+        b += own[j];
+    }
+    gone = lane_of(gone, lane);
+    return (hits ? 0 : kBins) + 8 * lane + __builtin_amdgcn_readlane(last, lane);
+}
+
 template <bool F16>
-__global__ __launch_bounds__(kDrawThreads) void k_draw_pick(const void *__restrict__ logits, int n, int P, bool aligned,
+__global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restrict__ logits, int n, int P,
                                                             const float *__restrict__ filter,
                                                             const float *__restrict__ rnd, uint32_t *__restrict__ token,
                                                             float *__restrict__ logp, DrawWork W) {
+    constexpr int NT = kPickThreads, NW = NT / 64;
+    using View = PieceView<F16, NT>;
     __shared__ PickShared S;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t row = blockIdx.x, base = row * n;
-    const DrawRow d = draw_row(filter + 4 * row, n);
     const uint64_t *hist = W.hist + row * P * kBins;
-    float u = rnd[row];
-    if (tid < P) S.piece[tid] = W.piece[row * P + tid];
-    if (!d.greedy) draw_table(S.tab);
+    // read ahead of the settings: rows without cuts leave them unused
+    uint4 ahead[kFew * kBins / 2 / NT];
+    if (P <= kFew) {
+#pragma unroll
+        for (int x = 0; x < kFew * kBins / 2 / NT; x++)
+            if (tid + NT * x < P * kBins / 2) ahead[x] = ((const uint4 *)hist)[tid + NT * x];
+    }
+    DrawHead mine_p{-INFINITY, 0, -kInfE, 0};
+    if (tid < P) {
+        const DrawPiece &q = W.piece[row * P + tid];
+        mine_p = DrawHead{q.m, q.idx, q.e, q.sum};
+    }
+    const DrawRow d = draw_row(filter + 4 * row, n);
+    const float u = rnd[row];
+    if (d.cuts && P <= kFew) {
+#pragma unroll
+        for (int x = 0; x < kFew * kBins / 2 / NT; x++) {
+            const bool in = tid + NT * x < P * kBins / 2;
+            ((uint4 *)S.hist)[tid + NT * x] = in ? ahead[x] : make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (!d.greedy) draw_table<NT>(S.tab);
+    if (tid < kMaxPieces) S.piece[tid] = mine_p;
     __syncthreads();
     float m = -INFINITY;
     double e = -kInfE;
     uint32_t first = 0xFFFFFFFFu;
-    for (int p = 0; p < P; p++) {
-        if (S.piece[p].m > m) m = S.piece[p].m, first = S.piece[p].idx;
-        e = fmax(e, S.piece[p].e);
+    for (int p0 = 0; p0 < P; p0 += 8) {
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            const DrawHead &q = S.piece[p0 + x];
+            if (q.m > m) m = q.m, first = q.idx;
+            e = fmax(e, q.e);
+        }
     }
     if (m == -INFINITY || d.greedy) {
         if (tid == 0) {
@@ -319,33 +476,41 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_pick(const void *__restri
         }
         return;
     }
-    // a piece's unit below the row's in octaves, and its first bin among the row's
-    auto octaves = [&](int p) { return (int)fmin((e - S.piece[p].e) * (1.0 / kSteps), 4000.0); };
-    auto shift = [&](int p) { return min(8 * octaves(p), kBins); };
+    if (tid < kMaxPieces) {
+        const int o = (int)fmin((e - mine_p.e) * (1.0 / kSteps), 4000.0);  // octaves below the row's
+        S.scale[tid] = o < 1000 ? ldexp(1.0, -o) : 0.0;
+        S.shift[tid] = mine_p.m > -INFINITY ? min(8 * o, kBins) : kBins;
+        S.kept[tid] = d.cuts ? 0 : mine_p.sum;
+    }
+    __syncthreads();
     const DrawUnit unit(d.c, e, m);
     const float low = draw_low(m, d);
+    const double inv_c = d.T * (0.69314718055994530942 / kSteps);
     DrawCut cut{0, 0xFFFFFFFFu};
     int cbin = kBins;  // the cut's bin; kBins: no cut
     if (d.cuts) {
-        if (tid < kBins) {
+        auto piece_bin = [&](int p, int b) { return P <= kFew ? S.hist[p * kBins + b] : hist[p * kBins + b]; };
+        for (int bin = tid; bin < kBins; bin += NT) {
             double s = 0.0;
             uint32_t c = 0;
             for (int p0 = 0; p0 < P; p0 += 8) {
                 uint64_t h[8];
+                if (P <= kFew) {
 #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    const int p = p0 + x, b = p < P && S.piece[p].m > -INFINITY ? tid - shift(p) : -1;
-                    h[x] = b >= 0 ? hist[p * kBins + b] : 0;
+                    for (int x = 0; x < 8; x++) h[x] = S.hist[x * kBins + max(bin - S.shift[x], 0)];
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 8; x++) h[x] = hist[min(p0 + x, P - 1) * kBins + max(bin - S.shift[p0 + x], 0)];
                 }
 #pragma unroll
                 for (int x = 0; x < 8; x++) {
-                    if (p0 + x >= P) break;
-                    s += ldexp((double)(h[x] & kSumMask), -octaves(p0 + x));
-                    c += (uint32_t)(h[x] >> 50);
+                    const uint64_t in = bin >= S.shift[p0 + x] ? h[x] : 0;  // past the last piece the shift is kBins
+                    s += (double)(in & kSumMask) * S.scale[p0 + x];
+                    c += (uint32_t)(in >> 50);
                 }
             }
-            S.sum[tid] = s;
-            S.cnt[tid] = c;
+            S.sum[bin_at(bin)] = s;
+            S.cnt[bin_at(bin)] = c;
         }
         if (d.min_p > 0.0f) {  // the smallest float whose weight is at least min_p
             const double lim = m == INFINITY ? INFINITY : (double)m + d.T * log((double)d.min_p);
@@ -358,18 +523,75 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_pick(const void *__restri
                 cbin = (unit.sharp ? kSharpDown : -unit.steps(f, r)) >> kBinShift;
             }
         }
-        // the keys of a bin into S.klo .. S.khi: its borders in l, exactly, from the floats around them
-        auto bin_keys = [&](int bin) {
-            __syncthreads();
-            if (wave == 0) {
-                if (unit.sharp) {
-                    if (lane == 0) S.klo = S.khi = lg_key(m);
-                } else {
+        // Stage 0: top-k (min-p has set its key already); stage 1: top-p of what
+        // that leaves.  Each finds the goal's bin, narrows its keys to one by
+        // passes over the bin's tokens (kNarrow), finds the last of that key's
+        // tokens if some have to go (kTies), and sums up what the pieces keep
+        // (kKeep).
+        enum { kNext, kNarrow, kTies, kKeep };
+        int mode = kNext, stage = -1, bin = 0, sh = 0;
+        uint32_t klo = 0, khi = 0, top_key = 0, cnt = 0, ties = 0, count = 0, ilo = 0, ihi = 0, step = 0;
+        uint64_t want = 0, before = 0;
+        bool limited = false;
+        DrawCut lim = cut;
+        int listed = -1;  // the bin in the list, with its keys from list_lo to list_hi
+        uint32_t list_lo = 0, list_hi = 0;
+        for (;;) {
+            const bool by_count = stage == 0;
+            if (mode == kNext) {
+                if (++stage == 2) break;
+                const bool counts = stage == 0;
+                if (counts ? d.top_k == 0 && cbin == kBins : d.top_p >= 1.0f) continue;
+                bool select = !counts || d.top_k;
+                double before_d = 0.0, goal = d.top_k;
+                __syncthreads();
+                if (select) {
+                    if (wave == 0) {
+                        double own[8], total = 0.0;
+                        bool some[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const int b = 8 * lane + j;
+                            own[j] = counts ? (double)S.cnt[bin_at(b)] : b < cbin ? S.sum[bin_at(b)] : 0.0;
+                            some[j] = own[j] > 0.0;
+                            total += own[j];
+                        }
+                        if (!counts) {  // of all that the cut so far leaves
+                            if (cbin < kBins) total = (double)S.kept[lane] * S.scale[lane] + (double)S.kept[lane + 64] * S.scale[lane + 64];
+                            goal = (double)d.top_p * lane_of(wave_scan(total), 63);
+                        }
+                        double gone = 0.0;
+                        int at = first_part(own, some, 0.0, goal, gone);
+                        if (at < 0 || at >= kBins) {  // not reached
+                            at = kBins;
+                            gone = 0.0;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) gone += own[j];
+                            gone = lane_of(wave_scan(gone), 63);
+                        }
+                        if (lane == 0) S.at = at, S.before_d = gone, S.before_u = __builtin_bit_cast(uint64_t, goal);
+                    }
+                    __syncthreads();
+                    bin = S.at;
+                    before_d = S.before_d;
+                    goal = __builtin_bit_cast(double, S.before_u);
+                    if (!counts && bin == kBins) bin = cbin;  // not above the cut's bin: in it
+                    // a count that ends below the cut, or among tokens without weight, cuts nothing
+                    select = bin <= cbin && bin < kDeepBin;
+                }
+                if (!select) {
+                    if (cbin == kBins) continue;
+                    bin = cbin;
+                }
+                // the bin's keys: its borders in l, exactly, from the floats around them
+                uint32_t low_key = lg_key(m);
+                top_key = low_key;
+                if (!unit.sharp) {
                     uint32_t at[2];
 #pragma unroll
                     for (int side = 0; side < 2; side++) {  // the first key of this bin, of the bin above
                         const int steps = (bin + 1 - side) << kBinShift;
-                        float f = (float)((e - steps + 0.5) / d.c);
+                        float f = (float)((e - steps + 0.5) * inv_c);
                         f = f == f ? fminf(fmaxf(f, kLeast), -kLeast) : 0.0f;
                         const uint32_t k0 = lg_key(f + 0.0f) - 32;
                         const float l = lg_unkey(k0 + lane);
@@ -377,312 +599,328 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw_pick(const void *__restri
                         const uint64_t yes = __ballot(l > m || (l >= low && -unit.steps(l, r) < steps));
                         at[side] = k0 + (yes ? __ffsll((long long)yes) - 1 : 64);
                     }
-                    if (lane == 0) S.klo = at[0], S.khi = min(at[1] - 1, lg_key(m));
+                    low_key = at[0];
+                    top_key = max(at[0], min(at[1] - 1, top_key));
                 }
-            }
-            __syncthreads();
-        };
-        // fn(key, index, logit) for a bin's tokens with keys in [klo, khi], from
-        // the pieces that have any, AT pieces in flight
-        auto row_pass = [&](auto at_c, int bin, uint32_t klo, uint32_t khi, auto fn) {
-            constexpr int AT = decltype(at_c)::value;
-            __syncthreads();
-            if (tid == 0) S.ntodo = 0;
-            __syncthreads();
-            if (tid < P) {
-                const int b = bin - shift(tid);
-                if (S.piece[tid].m > -INFINITY && b >= 0 && hist[tid * kBins + b]) S.todo[atomicAdd(&S.ntodo, 1)] = tid;
-            }
-            __syncthreads();
-            const float llo = lg_unkey(klo), lhi = lg_unkey(khi);
-            for (int t = 0; t < S.ntodo; t += AT) {
-                float v[AT][kPer];
-#pragma unroll
-                for (int a = 0; a < AT; a++)
-                    if (t + a < S.ntodo) piece_load<F16>(logits, base, S.todo[t + a] * kPiece, n, aligned, v[a]);
-#pragma unroll
-                for (int a = 0; a < AT; a++) {
-                    if (t + a >= S.ntodo) break;
-                    const int i0 = S.todo[t + a] * kPiece;
-#pragma unroll
-                    for (int x = 0; x < kPer; x++)
-                        if (v[a][x] >= llo && v[a][x] <= lhi) fn(lg_key(v[a][x]), (uint32_t)(i0 + piece_token<F16>(aligned, x)));
-                }
-            }
-        };
-        int listed = -1;  // the bin in the list, with its keys from list_lo to list_hi
-        uint32_t list_lo = 0, list_hi = 0;
-        auto holds = [&](int bin, uint32_t klo, uint32_t khi) { return listed == bin && klo >= list_lo && khi <= list_hi; };
-        auto bin_pass = [&](int bin, uint32_t klo, uint32_t khi, auto fn) {
-            if (holds(bin, klo, khi)) {
-                for (uint32_t i = tid; i < S.list_n; i += kDrawThreads) {
-                    const uint32_t k = S.list_key[i];
-                    if (k >= klo && k <= khi) fn(k, S.list_idx[i]);
-                }
-            } else {
-                row_pass(std::integral_constant<int, 1>{}, bin, klo, khi, fn);
-            }
-        };
-        // stage 0: top-k (min-p has set its key already); stage 1: top-p of what that leaves
-        for (int stage = 0; stage < 2; stage++) {
-            const bool by_count = stage == 0;
-            if (by_count ? d.top_k == 0 && cbin == kBins : d.top_p >= 1.0f) continue;
-            if (!by_count || d.top_k) {
-                double goal = d.top_k;
-                if (!by_count) {
-                    double s = 0.0;
-                    if (cbin < kBins)
-                        for (int p = tid; p < P; p += kDrawThreads) s += ldexp((double)S.kept[p], -octaves(p));
-                    else if (tid < kBins)
-                        s = S.sum[tid];
-                    s = wave_sum(s);
-                    __syncthreads();
-                    if (lane == 0) S.red[wave] = s;
-                    __syncthreads();
-                    goal = 0.0;
-                    for (int w = 0; w < 16; w++) goal += S.red[w];
-                    goal *= (double)d.top_p;
-                }
-                // the first bin at which the running count or sum reaches the goal
-                __syncthreads();
-                if (wave == 0) {
-                    double own[8], s = 0.0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int b = 8 * lane + j;
-                        own[j] = by_count ? (double)S.cnt[b] : b < cbin ? S.sum[b] : 0.0;
-                        s += own[j];
-                    }
-                    double run = s;
-                    for (int o = 1; o < 64; o <<= 1) {
-                        const double x = __shfl_up(run, o);
-                        if (lane >= o) run += x;
-                    }
-                    const uint64_t hit = __ballot(run >= goal && run > 0.0);
-                    if (hit == 0 && lane == 63) S.at = kBins, S.before_d = run;
-                    if (hit && lane == __ffsll((long long)hit) - 1) {
-                        double b = run - s, last_b = b;
-                        int last = 0;
-                        bool done = false;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            if (!done && own[j] > 0.0) last = j, last_b = b;
-                            done = done || (own[j] > 0.0 && b + own[j] >= goal);
-                            b += own[j];
-                        }
-                        S.at = 8 * lane + last;
-                        S.before_d = last_b;
-                    }
-                }
-                __syncthreads();
-                int bin = S.at;
-                const double before_d = S.before_d;
-                if (!by_count && bin == kBins) bin = cbin;  // not above the cut's bin: in it
-                // a count that ends below the cut, or among tokens without weight, cuts nothing
-                if (bin <= cbin && bin < kDeepBin) {
-                    const bool limited = bin == cbin;
-                    const DrawCut lim = cut;
-                    bin_keys(bin);
-                    const uint32_t klo0 = limited ? max(S.klo, lim.key) : S.klo;
-                    uint32_t klo = klo0, khi = max(S.khi, klo0);
+                cnt = S.cnt[bin_at(bin)];
+                if (select) {
+                    limited = bin == cbin;
+                    lim = cut;
+                    klo = limited ? max(low_key, lim.key) : low_key;
+                    khi = max(top_key, klo);
                     // the goal inside the bin: a count, or weights kInBits below the octave that holds the bin's top
                     const double left = fmax(goal - before_d, 0.0);
-                    const uint64_t want = by_count ? (uint64_t)left : (uint64_t)ceil(ldexp(left, (bin >> 3) + kInBits - kCutBits));
-                    const DrawUnit in_unit(d.c, e - (double)kSteps * (bin >> 3), m);
-                    uint64_t before = 0;
-                    uint32_t cnt = S.cnt[bin], ties = 0;
-                    for (;;) {  // keys are narrowed by 512 parts of their range until one is left
-                        if (cnt <= kList && !holds(bin, klo, khi)) {
-                            __syncthreads();
-                            if (tid == 0) S.list_n = 0;
-                            row_pass(std::integral_constant<int, 4>{}, bin, klo, khi, [&](uint32_t k, uint32_t i) {
-                                const uint32_t x = atomicAdd(&S.list_n, 1u);
-                                if (x < kList) S.list_key[x] = k, S.list_idx[x] = i;
-                            });
-                            __syncthreads();
-                            listed = S.list_n <= kList ? bin : -1;
-                            list_lo = klo;
-                            list_hi = khi;
-                        }
-                        int sh = 0;
-                        while ((khi - klo) >> sh >= kBins) sh++;
-                        __syncthreads();
-                        if (tid < kBins) S.sub_sum[tid] = 0, S.sub_cnt[tid] = 0;
-                        __syncthreads();
-                        bin_pass(bin, klo, khi, [&](uint32_t k, uint32_t i) {
-                            if (limited && !lim.keeps(k, i)) return;
-                            const uint32_t b = (khi - k) >> sh;
-                            int down;
-                            atomicAdd(&S.sub_cnt[b], 1u);
-                            if (!by_count)
-                                atomicAdd((unsigned long long *)&S.sub_sum[b], (unsigned long long)draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down));
-                        });
-                        __syncthreads();
-                        if (wave == 0) {
-                            uint64_t own[8], s = 0;
-                            uint32_t c[8], some = 0;
+                    want = counts ? (uint64_t)left : (uint64_t)ceil(ldexp(left, (bin >> 3) + kInBits - kCutBits));
+                    before = 0;
+                    mode = kNarrow;
+                } else {
+                    mode = kKeep;
+                }
+                if (mode == kNarrow) continue;
+            }
+            if (mode == kKeep) {  // whole bins; the cut's own token by token
+                for (int p = wave; p < P; p += NW) {
+                    uint64_t s = 0;
+                    const int top = cbin - S.shift[p];
 #pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                c[j] = S.sub_cnt[8 * lane + j];
-                                own[j] = by_count ? c[j] : S.sub_sum[8 * lane + j];
-                                some |= c[j];
-                                s += own[j];
-                            }
-                            uint64_t run = s;
-                            for (int o = 1; o < 64; o <<= 1) {
-                                const uint64_t x = __shfl_up(run, o);
-                                if (lane >= o) run += x;
-                            }
-                            if (lane == 0) S.at = 0, S.ties = 0, S.before_u = before;  // stands if the range is empty
-                            const uint64_t any = __ballot(some != 0), hit = __ballot(some != 0 && before + run >= want);
-                            if (lane == (hit ? __ffsll((long long)hit) : 64 - __clzll((long long)any)) - 1) {
-                                uint64_t b = before + run - s, last_b = b;
-                                uint32_t last = 0, last_c = 0;
-                                bool done = false;
+                    for (int x = 0; x < kBins; x += 64) s += x + lane < top ? piece_bin(p, x + lane) & kSumMask : 0;
+                    s = wave_scan(s);
+                    if (lane == 63) S.kept[p] = s;
+                }
+                klo = cut.key;
+                khi = max(top_key, klo);
+            } else if (mode == kNarrow) {
+                sh = 0;
+                while ((khi - klo) >> sh >= kBins) sh++;
+            } else {
+                step = (ihi - ilo) / kBins + 1;
+            }
+            // a pass over the bin's tokens with keys in [klo, khi]: from the list,
+            // into which a bin of at most kList tokens goes whole, a larger one
+            // half a piece at a time
+            const bool held = listed == bin && klo >= list_lo && khi <= list_hi;
+            __syncthreads();
+            if (mode != kKeep)
+                for (int b = tid; b < kBinRoom; b += NT) S.sub_sum[b] = 0, S.sub_cnt[b] = 0;
+            if (tid == 0) S.ntodo = 0, S.list_n = held ? S.list_n : 0;
+            __syncthreads();
+            int chunks = 1;
+            if (!held) {
+                if (tid < P) {
+                    const int b = bin - S.shift[tid];
+                    if (b >= 0 && piece_bin(tid, b)) S.todo[atomicAdd(&S.ntodo, 1)] = tid;
+                }
+                __syncthreads();
+                listed = -1;
+                if (cnt <= kList)
+                    listed = bin, list_lo = klo, list_hi = khi;
+                else
+                    chunks = 2 * S.ntodo;  // kListRoom tokens each at most
+            }
+            const DrawUnit in_unit(d.c, e - (double)kSteps * (bin >> 3), m);
+            for (int ch = 0; ch < chunks; ch++) {
+                if (!held) {
+                    const int t0 = listed >= 0 ? 0 : ch >> 1, t1 = listed >= 0 ? S.ntodo : t0 + 1;
+                    // the masks below hold 16 tokens of a thread: of a piece's 32 and a vector, half a piece is the first
+                    constexpr int kMask = 16;
+                    auto ch_mask = [&](int x0) { return listed >= 0 || (x0 >= kMask) == (ch & 1) ? ~0u : 0u; };
+                    const float llo = lg_unkey(klo), lhi = lg_unkey(khi);
+                    if (ch) {
+                        __syncthreads();
+                        if (tid == 0) S.list_n = 0;
+                        __syncthreads();
+                    }
+                    constexpr int AT = 4;  // pieces in flight
+                    for (int t = t0; t < t1; t += AT) {
+                        uint4 raw[AT][View::NV];
 #pragma unroll
-                                for (int j = 0; j < 8; j++) {
-                                    if (!done && c[j]) last = j, last_c = c[j], last_b = b;
-                                    done = done || (c[j] && b + own[j] >= want);
-                                    b += own[j];
+                        for (int a = 0; a < AT; a++)
+                            if (t + a < t1) View(logits, base, S.todo[t + a], n).load(raw[a]);
+#pragma unroll
+                        for (int a = 0; a < AT; a++) {
+                            if (t + a >= t1) break;
+                            const View view(logits, base, S.todo[t + a], n);
+                            view.edges(raw[a]);
+#pragma unroll
+                            for (int x0 = 0; x0 < View::N; x0 += kMask) {
+                                constexpr int M = kMask;
+                                uint32_t hits = 0;  // tokens in the range, the first one in the highest bit
+#pragma unroll
+                                for (int x = x0; x < x0 + M && x < View::N; x++) {
+                                    const float l = raw_value<F16>(raw[a][x / View::V], x % View::V);
+                                    hits = hits + hits + (__builtin_amdgcn_fmed3f(l, llo, lhi) == l);  // a NaN is not
                                 }
-                                S.at = 8 * lane + last;
-                                S.ties = last_c;
-                                S.before_u = last_b;
+                                hits &= ch_mask(x0);
+                                while (hits) {
+                                    const int z = __clz((int)hits), x = x0 + z - (32 - min(M, View::N - x0));
+                                    hits &= ~(0x80000000u >> z);
+                                    const uint32_t at = atomicAdd(&S.list_n, 1u);
+                                    if (at < kListRoom) S.list_idx[at] = view.token(x);
+                                }
                             }
                         }
-                        __syncthreads();
-                        before = S.before_u;
-                        cnt = ties = S.ties;
-                        khi -= S.at << sh;
-                        if (sh == 0) break;
-                        klo = max(klo, khi - ((1u << sh) - 1u));
                     }
-                    // one key is left; its tokens weigh the same, so a division tells how many stay
+                    __syncthreads();
+                }
+                const uint32_t have = min(S.list_n, (uint32_t)kListRoom);
+                if (!held)  // their keys, all loads at once; below a thread meets its own
+                    for (uint32_t x = tid; x < have; x += NT) S.list_key[x] = lg_key(lg_value<F16>(logits, base + S.list_idx[x]));
+                for (uint32_t x = tid; x < have; x += NT) {
+                    const uint32_t k = S.list_key[x], i = S.list_idx[x];
+                    if (k < klo || k > khi) continue;
+                    if (mode == kTies) {
+                        if (i >= ilo && i <= ihi) atomicAdd(&S.sub_cnt[bin_at((i - ilo) / step)], 1u);
+                        continue;
+                    }
+                    const bool keep = mode == kKeep;
+                    if (keep ? !cut.keeps(k, i) : limited && !lim.keeps(k, i)) continue;
+                    const int part = bin_at((int)((khi - k) >> sh)), p = i / kPiece;
+                    if (!keep) atomicAdd(&S.sub_cnt[part], 1u);
+                    if (!keep && by_count) continue;
                     int down;
-                    const uint64_t w = by_count ? 1 : draw_weight(in_unit, lg_unkey(khi), kInBits, S.tab, down);
-                    uint32_t c = want > before && w ? (uint32_t)min((unsigned long long)((want - before + w - 1) / w), (unsigned long long)n) : 1;
-                    cut = DrawCut{khi, limited && lim.key == khi ? lim.last : 0xFFFFFFFFu};
-                    cbin = bin;
-                    if (c < ties) {  // the index of the c-th token of this key, by 512 parts of the index range
-                        uint32_t lo = 0, hi = (uint32_t)n - 1;
-                        while (lo < hi) {
-                            const uint32_t step = (hi - lo) / kBins + 1;
-                            __syncthreads();
-                            if (tid < kBins) S.sub_cnt[tid] = 0;
-                            __syncthreads();
-                            bin_pass(bin, khi, khi, [&](uint32_t, uint32_t i) {
-                                if (i >= lo && i <= hi) atomicAdd(&S.sub_cnt[(i - lo) / step], 1u);
-                            });
-                            __syncthreads();
-                            if (tid == 0) {
-                                uint32_t b = 0, got = 0;
-                                while (b < kBins - 1 && got + S.sub_cnt[b] < c) got += S.sub_cnt[b++];
-                                S.at = b;
-                                S.ties = got;
-                            }
-                            __syncthreads();
-                            c -= S.ties;
-                            lo += S.at * step;
-                            hi = min(hi, lo + step - 1);
-                        }
-                        cut.last = lo;
-                    }
+                    const DrawUnit to = keep ? DrawUnit(d.c, S.piece[p].e, S.piece[p].m) : in_unit;
+                    const uint64_t w = draw_weight(to, lg_unkey(k), keep ? kCutBits : kInBits, S.tab, down);
+                    atomicAdd((unsigned long long *)(keep ? &S.kept[p] : &S.sub_sum[part]), (unsigned long long)w);
                 }
             }
-            if (cbin == kBins) continue;
-            // kept sums of the pieces: whole bins, and the cut's own bin token by token
-            bin_keys(cbin);
-            for (int p = wave; p < P; p += 16) {
-                uint64_t s = 0;
-                const int top = S.piece[p].m > -INFINITY ? cbin - shift(p) : 0;
+            __syncthreads();
+            if (mode == kKeep) {
+                mode = kNext;
+            } else if (mode == kNarrow) {
+                if (wave == 0) {
+                    uint64_t own[8], gone = before;
+                    uint32_t c[8];
+                    bool some[8];
 #pragma unroll
-                for (int x = 0; x < kBins; x += 64) s += x + lane < top ? hist[p * kBins + x + lane] & kSumMask : 0;
-                s = wave_sum(s);
-                if (lane == 0) S.kept[p] = s;
+                    for (int j = 0; j < 8; j++) {
+                        c[j] = S.sub_cnt[9 * lane + j];
+                        own[j] = by_count ? c[j] : S.sub_sum[9 * lane + j];
+                        some[j] = c[j] != 0;
+                    }
+                    const int at = first_part(own, some, before, want, gone);
+                    if (lane == 0) S.at = at < 0 ? 0 : at & (kBins - 1), S.before_u = gone, S.ties = at < 0 ? 0 : S.sub_cnt[bin_at(at & (kBins - 1))];
+                }
+                __syncthreads();
+                before = S.before_u;
+                cnt = ties = S.ties;
+                khi -= S.at << sh;
+                if (sh) {
+                    klo = max(klo, khi - ((1u << sh) - 1u));
+                } else {
+                    // one key is left; its tokens weigh the same, so a division tells how many stay
+                    const uint64_t left = want > before ? want - before : 0;
+                    const uint64_t w = by_count ? 1 : (uint64_t)rint((double)S.sub_sum[bin_at(S.at)] / (double)max(ties, 1u));
+                    count = w ? (uint32_t)fmin(ceil((double)left / (double)w), (double)n) : 1;
+                    if (count * w < left) count++;  // the division's rounding
+                    else if (count && (count - 1) * w >= left) count--;
+                    count = max(count, 1u);
+                    klo = khi;
+                    cut = DrawCut{khi, limited && lim.key == khi ? lim.last : 0xFFFFFFFFu};
+                    cbin = bin;
+                    cnt = S.cnt[bin_at(bin)];
+                    mode = count < ties ? kTies : kKeep;
+                    ilo = 0;
+                    ihi = n - 1;
+                }
+            } else {
+                if (tid == 0) {
+                    uint32_t b = 0, got = 0;
+                    while (b < kBins - 1 && got + S.sub_cnt[bin_at(b)] < count) got += S.sub_cnt[bin_at(b++)];
+                    S.at = b;
+                    S.ties = got;
+                }
+                __syncthreads();
+                count -= S.ties;
+                ilo += S.at * step;
+                ihi = min(ihi, ilo + step - 1);
+                if (ilo >= ihi) {
+                    cut.last = ilo;
+                    mode = kKeep;
+                }
             }
-            const uint32_t top_key = S.khi;
-            __syncthreads();
-            bin_pass(cbin, cut.key, top_key, [&](uint32_t k, uint32_t i) {
-                if (!cut.keeps(k, i)) return;
-                const int p = i / kPiece;
-                const DrawUnit pu(d.c, S.piece[p].e, S.piece[p].m);
-                int down;
-                atomicAdd((unsigned long long *)&S.kept[p], (unsigned long long)draw_weight(pu, lg_unkey(k), kCutBits, S.tab, down));
-            });
+        }
+        if (cbin == kBins) {  // nothing was cut
+            for (int p = wave; p < P; p += NW) {
+                uint64_t s = 0;
+                if (S.shift[p] < kBins || S.scale[p] > 0.0)
+#pragma unroll
+                    for (int x = 0; x < kBins; x += 64) s += piece_bin(p, x + lane) & kSumMask;
+                s = wave_scan(s);
+                if (lane == 63) S.kept[p] = s;
+            }
             __syncthreads();
         }
     }
-    // Where no cut was found (all tokens stay) a row with cuts has its sums in the bins.
+    // the draw's piece: every wave goes through them, the same way
     const int bits = d.cuts ? kCutBits : kPlainBits;
-    if (cbin == kBins) {
-        for (int p = wave; p < P; p += 16) {
-            uint64_t s = S.piece[p].sum;
-            if (d.cuts) {
-                s = 0;
-                if (S.piece[p].m > -INFINITY)
-                    for (int x = lane; x < kBins; x += 64) s += hist[p * kBins + x] & kSumMask;
-                s = wave_sum(s);
-            }
-            if (lane == 0) S.kept[p] = s;
-        }
-        __syncthreads();
-    }
-    // the draw's piece
     double total = 0.0;
-    for (int p = 0; p < P; p++) total += ldexp((double)S.kept[p], -octaves(p));
-    u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
-    const double target = (double)u * total;
-    double run = 0.0, at = 0.0;
-    int piece = 0;
-    for (int p = 0; p < P; p++) {
-        if (S.kept[p] == 0) continue;
-        piece = p;
-        at = run;
-        run += ldexp((double)S.kept[p], -octaves(p));
-        if (run > target) break;
+    for (int p0 = 0; p0 < P; p0 += 8) {
+#pragma unroll
+        for (int x = 0; x < 8; x++) total += (double)S.kept[p0 + x] * S.scale[p0 + x];
     }
-    // its token: lanes hold tokens of the piece in index order
+    const double target = (double)(u > 0.0f ? fminf(u, 1.0f) : 0.0f) * total;
+    double run = 0.0, gone = 0.0;
+    int piece = -1;
+    for (int p0 = 0; p0 < P; p0 += 8) {
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            const double s = (double)S.kept[p0 + x] * S.scale[p0 + x];
+            if (s > 0.0 && run <= target) piece = p0 + x, gone = run;
+            run += s;
+        }
+    }
+    // ln of the kept sum beside the maximum: total 2^(E - bits), the maximum
+    // lies `below` octaves under E
+    double below = 1.0;
+    if (!unit.sharp) {
+        double r;
+        below = -(double)unit.steps(m, r);
+        below = (below - r) / kSteps;
+    }
     const DrawUnit pu(d.c, S.piece[piece].e, S.piece[piece].m);
     const float plow = draw_low(S.piece[piece].m, d);
-    uint64_t goal = (uint64_t)fmax(ldexp(target - at, octaves(piece)), 0.0);
+    uint64_t goal = (uint64_t)fmax((target - gone) / S.scale[piece], 0.0);
     if (goal >= S.kept[piece]) goal = S.kept[piece] - 1;
-    float v[kPer];
-    uint64_t w[kPer], mine = 0;
-    const int i0 = piece * kPiece + tid * kPer;
-#pragma unroll
-    for (int x = 0; x < kPer; x++) v[x] = i0 + x < n ? lg_value<F16>(logits, base + i0 + x) : -INFINITY;
-#pragma unroll
-    for (int x = 0; x < kPer; x++) {
+    // The token.  A plain row's piece has sums by groups of 1024 tokens (where
+    // the row starts at a 16-byte border), and threads take four tokens of the
+    // group each.  Otherwise they take 32 of the piece through LDS and weigh
+    // those that are kept.
+    const bool grouped = !d.cuts && base % View::V == 0;
+    auto weight = [&](float l) {
         int down;
-        w[x] = 0;
-        if (v[x] >= plow && cut.keeps(lg_key(v[x]), i0 + x)) w[x] = draw_weight(pu, v[x], bits, S.tab, down);
-        mine += w[x];
-    }
-    uint64_t pre = mine;
-    for (int s = 1; s < 64; s <<= 1) {
-        const uint64_t o = __shfl_up(pre, s);
-        if (lane >= s) pre += o;
-    }
-    uint64_t *wave_total = S.sub_sum;
-    if (lane == 63) wave_total[wave] = pre;
-    __syncthreads();
-    uint64_t b = pre - mine;
-    for (int x = 0; x < wave; x++) b += wave_total[x];
-    if (goal >= b && goal < b + mine) {
-        int hit = -1;
-        float l = 0.0f;
+        return draw_weight(pu, l, bits, S.tab, down);
+    };
+    auto find = [&](uint64_t mine, uint64_t b, auto walk) {  // walk(up to): the token of a thread's own at which its sum passes it
+        const uint64_t pre = wave_scan(mine);
+        if (lane == 63) S.wave_total[wave] = pre;
+        __syncthreads();
+        b += pre - mine;
 #pragma unroll
-        for (int x = 0; x < kPer; x++) {
-            b += w[x];
-            if (hit < 0 && goal < b) hit = x, l = v[x];
+        for (int y = 0; y < NW; y++)
+            if (y < wave) b += S.wave_total[y];
+        if (goal < b || goal >= b + mine) return;
+        float l;
+        token[row] = walk(goal - b, l);
+        if (logp) logp[row] = (float)((l == m ? 0.0 : ((double)l - (double)m) / d.T) - (log(ldexp(total, -bits)) + below * 0.69314718055994530942));
+    };
+    if (grouped) {
+        constexpr int V = 4;
+        static_assert(kGroup == NT * V);
+        const uint64_t *group = W.piece[row * P + piece].group;
+        uint64_t gs[kGroups], b = 0, run_g = 0;
+        int g = 0;
+#pragma unroll
+        for (int x = 0; x < kGroups; x++) gs[x] = group[x];
+#pragma unroll
+        for (int x = 0; x < kGroups; x++) {
+            if (run_g <= goal) g = x, b = run_g;
+            run_g += gs[x];
         }
-        token[row] = i0 + hit;
-        if (logp) {  // the sum is total 2^(E - bits); the maximum lies `below` octaves under E
-            double r = 0.0, below = 1.0;
-            if (!unit.sharp) below = -(unit.steps(m, r) + 0.0) / kSteps, below -= r / kSteps;
-            const double z = l == m ? 0.0 : ((double)l - (double)m) / d.T;
-            logp[row] = (float)(z - (log(ldexp(total, -bits)) + below * 0.69314718055994530942));
+        const int i0 = piece * kPiece + g * kGroup + tid * V;
+        float v[V];
+        uint64_t w[V], mine = 0;
+#pragma unroll
+        for (int x = 0; x < V; x++) v[x] = i0 + x < n ? lg_value<F16>(logits, base + i0 + x) : -INFINITY;
+#pragma unroll
+        for (int x = 0; x < V; x++) w[x] = v[x] >= plow ? weight(v[x]) : 0, mine += w[x];
+        find(mine, b, [&](uint64_t left, float &l) {
+            int hit = V - 1;
+            l = v[V - 1];
+            uint64_t up = mine;
+#pragma unroll
+            for (int x = V - 1; x >= 0; x--) {
+                if (left < up && w[x]) hit = x, l = v[x];
+                up -= w[x];
+            }
+            return (uint32_t)(i0 + hit);
+        });
+    } else {
+        const float lc = cbin == kBins ? plow : lg_unkey(cut.key);  // kept: above it, or at it up to index cut.last
+        const View view(logits, base, piece, n);
+        uint4 raw[View::NV];
+        view.load(raw);
+        float v[View::N];
+        view.values(raw, v);
+        // position j of the view (token view.first + j) at j + 4 (j / 32): 16-byte writes and reads, all banks
+#pragma unroll
+        for (int x = 0; x < View::N; x += 4) {
+            const int j = (tid + NT * (x / View::V)) * View::V + x % View::V;
+            if (j < kPiece + 8) *(float4 *)&S.tok[j + 4 * (j >> 5)] = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
         }
+        __syncthreads();
+        constexpr int PT = kPiece / NT;
+        const uint32_t i0 = view.first + tid * PT;
+        const float4 *own4 = (const float4 *)(S.tok + (PT + 4) * tid);
+        const float *own = (const float *)own4;
+        uint32_t keep = 0, more = 0;
+#pragma unroll
+        for (int x = 0; x < PT; x += 4) {
+            const float4 q = own4[x / 4];
+            const float l[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int y = 0; y < 4; y++) keep |= l[y] > lc || (l[y] == lc && i0 + x + y <= cut.last) ? 1u << (x + y) : 0;
+        }
+        // the last thread has the tokens behind the last border too
+        if (view.off && tid == NT - 1)
+            for (int x = 0; x < 8; x++) {
+                const float l = own[PT + 4 + x];
+                more |= l > lc || (l == lc && i0 + PT + x <= cut.last) ? 1u << x : 0;
+            }
+        uint64_t mine = 0;
+        for (uint32_t k = keep; k; k &= k - 1) mine += weight(own[__ffs((int)k) - 1]);
+        for (uint32_t k = more; k; k &= k - 1) mine += weight(own[PT + 3 + __ffs((int)k)]);
+        find(mine, 0, [&](uint64_t left, float &l) {
+            uint64_t up = 0;
+            int x = 0;
+            for (uint32_t k = keep, z = 0; z < 2; k = more, z++) {
+                for (; k && left >= up; k &= k - 1) {
+                    x = __ffs((int)k) - 1 + (z ? PT : 0);
+                    l = own[x + 4 * (x / PT)];
+                    up += weight(l);
+                }
+            }
+            return i0 + x;
+        });
     }
 }
 
@@ -831,10 +1069,10 @@ uint64_t logits_work_words(uint64_t n, uint64_t rows) {
 }
 
 template <bool F16>
-static void draw_launch(rsv_ctx *ctx, const void *logits, int n, int P, bool aligned, const float *filter, const float *rnd,
+static void draw_launch(rsv_ctx *ctx, const void *logits, int n, int P, const float *filter, const float *rnd,
                         uint32_t *token, float *logp, const DrawWork &W, uint64_t rows) {
-    hipLaunchKernelGGL((k_draw_scan<F16>), dim3((unsigned)(rows * P)), dim3(kDrawThreads), 0, ctx->stream, logits, n, P, aligned, filter, W);
-    hipLaunchKernelGGL((k_draw_pick<F16>), dim3((unsigned)rows), dim3(kDrawThreads), 0, ctx->stream, logits, n, P, aligned, filter, rnd,
+    hipLaunchKernelGGL((k_draw_scan<F16>), dim3((unsigned)(rows * P)), dim3(kScanThreads), 0, ctx->stream, logits, n, P, filter, W);
+    hipLaunchKernelGGL((k_draw_pick<F16>), dim3((unsigned)rows), dim3(kPickThreads), 0, ctx->stream, logits, n, P, filter, rnd,
                        token, logp, W);
 }
 
@@ -844,11 +1082,10 @@ int launch_draw(rsv_ctx *ctx, const void *logits, int f16, uint32_t *token, uint
     DrawWork W;
     W.hist = (uint64_t *)work;
     W.piece = (DrawPiece *)(W.hist + rows * P * kBins);
-    const bool aligned = n * (f16 ? 2 : 4) % 16 == 0;
     if (f16)
-        draw_launch<true>(ctx, logits, (int)n, P, aligned, filter, rnd, token, logp, W, rows);
+        draw_launch<true>(ctx, logits, (int)n, P, filter, rnd, token, logp, W, rows);
     else
-        draw_launch<false>(ctx, logits, (int)n, P, aligned, filter, rnd, token, logp, W, rows);
+        draw_launch<false>(ctx, logits, (int)n, P, filter, rnd, token, logp, W, rows);
     RSV_HIP(hipGetLastError());
     return 0;
 }

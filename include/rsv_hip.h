@@ -497,7 +497,8 @@ int rsv_wkv7_lora_decode(rsv_ctx *ctx, const rsv_wkv_lora *op, uint64_t batch);
  * decoded token per session, packed prompts, or both.  Rows that stand
  * together share the adapter's reads.
  *
- * k, n and rank are multiples of 8 (16-byte fp16 rows), rank at most 128.
+ * k, n (at most 4194304) and rank (at most 128) are multiples of 8: fp16 rows
+ * of 16 bytes.
  * epilogue: 0 (store) or 3 (relu^2), as rsv_gemm_ex.  out may be y itself;
  * otherwise no job's out may be an operand of the call.  Products and sums
  * are fp32 whatever the operands' types (an F16 out is rounded once).

@@ -1755,7 +1755,7 @@ static int real_opnd(rsv_ctx *ctx, uint32_t id, uint64_t min_len, void **p, int 
     return 0;
 }
 
-constexpr uint64_t kAdapterRows = (uint64_t)1 << 20, kAdapterDim = (uint64_t)1 << 24, kAdapterRank = 128;
+constexpr uint64_t kAdapterRows = (uint64_t)1 << 20, kAdapterDim = (uint64_t)1 << 22, kAdapterRank = 128;
 
 // The limits of rsv_adapter_multi that do not need a context.
 static int adapter_limits(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows) {

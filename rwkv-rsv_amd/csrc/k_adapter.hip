@@ -17,7 +17,10 @@
 namespace rsv {
 
 typedef _Float16 ad_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ad_h4 __attribute__((ext_vector_type(4)));
 typedef float ad_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ad_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ad_u2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWin = 64;
 constexpr int kBare = -1;  // the group of a window's rows without an adapter
@@ -88,12 +91,33 @@ __device__ __forceinline__ AdGroup ad_group(const AdWindow &w, int g) {
     return r;
 }
 
-__device__ __forceinline__ float ad_load(const void *p, int f16, size_t i) {
-    return f16 ? (float)((const _Float16 *)p)[i] : ((const float *)p)[i];
-}
-
 __device__ __forceinline__ float ad_epi(float z, int epi) {
     return epi == GE_RELU2 ? (z > 0.0f ? z * z : z == z ? 0.0f : z) : z;
+}
+
+// Memory through buffer resources: an offset past the size reads as zero and
+// is not written, so tails, masked rows and ranks past an adapter's own need
+// no branches around the loads.  A resource covers one adapter's matrix or one
+// window's rows, at most 2^30 bytes; kOff added to an offset below that, once
+// or twice, stays past every size.
+constexpr uint32_t kOff = 0x40000000u;
+struct AdBuf {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ AdBuf(const void *p, size_t bytes) : r(__builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, (int)bytes, 0x00020000)) {}
+    __device__ __forceinline__ ad_h8 h8(uint32_t at) const { return __builtin_bit_cast(ad_h8, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); }
+    __device__ __forceinline__ ad_f4 f4(uint32_t at) const { return __builtin_bit_cast(ad_f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); }
+    __device__ __forceinline__ ad_h4 h4(uint32_t at) const { return __builtin_bit_cast(ad_h4, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0)); }
+    __device__ __forceinline__ float f1(uint32_t at) const { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0)); }
+    __device__ __forceinline__ float h1(uint32_t at) const { return (float)__builtin_bit_cast(_Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0)); }
+    __device__ __forceinline__ void put(ad_f4 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ad_u4, v), r, at, 0, 0); }
+    __device__ __forceinline__ void put(ad_h4 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(ad_u2, v), r, at, 0, 0); }
+    __device__ __forceinline__ void put(float v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), r, at, 0, 0); }
+    __device__ __forceinline__ void put(_Float16 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), r, at, 0, 0); }
+};
+// A window's rows of [rows, n].
+__device__ __forceinline__ AdBuf ad_rows(const AdapterJobs &J, const void *p, int n, int f16, int win) {
+    const size_t row = (size_t)n * (f16 ? 2 : 4);
+    return AdBuf((const char *)p + (size_t)win * kWin * row, min(kWin, J.rows - win * kWin) * row);
 }
 
 // Products of a 16-rank tile with MT 16-row tiles over k in [k0, k1), one
@@ -101,37 +125,40 @@ __device__ __forceinline__ float ad_epi(float z, int epi) {
 // Lane (i = l%16, g = l/16) supplies k 8g..8g+7 of each 32: the rank rows as
 // the left operand, the batch rows as the right one.  fp16 x goes through
 // v_mfma_f32_16x16x32_f16 (products of fp16 are exact in fp32), fp32 x through
-// eight v_mfma_f32_16x16x4_f32 with A widened, so both sum in fp32.
+// eight v_mfma_f32_16x16x4_f32 with A widened, so both sum in fp32.  DEP steps
+// of 32 k are in flight at once.  xrow: byte offsets of the rows (kOff: none).
 template <int RT, int MT, bool X16, int DEP>
-__device__ __forceinline__ void ad_dots(const _Float16 *__restrict__ A, const void *__restrict__ x, const size_t (&xrow)[MT],
-                                        const bool (&live)[MT], int R, int K, int k0, int k1, ad_f4 (&acc)[MT][RT]) {
+__device__ __forceinline__ void ad_dots(const AdBuf &A, const AdBuf &x, const uint32_t (&xrow)[MT], int K, int k0, int k1,
+                                        ad_f4 (&acc)[MT][RT]) {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    constexpr ad_h8 zero = {};
+    uint32_t arow[RT];
+#pragma unroll
+    for (int j = 0; j < RT; j++) arow[j] = (16 * j + i) * K * 2u;
     for (int kb = k0; kb < k1; kb += 32 * DEP) {
         ad_h8 a[DEP][RT];
         ad_h8 xh[DEP][MT];
         ad_f4 xf[DEP][MT][2];
 #pragma unroll
         for (int s = 0; s < DEP; s++) {
-            const int k = kb + 32 * s + 8 * g;
-            const bool in = k < k1;
+            if (kb + 32 * s >= k1) break;
+            const uint32_t k = kb + 32 * s + 8 * g;
+            const bool in = (int)k < k1;
+            const uint32_t ka = in ? 2 * k : 2 * kOff, kx = in ? (X16 ? 2 : 4) * k : 2 * kOff;
 #pragma unroll
-            for (int j = 0; j < RT; j++)
-                a[s][j] = in && 16 * j + i < R ? *(const ad_h8 *)(A + (size_t)(16 * j + i) * K + k) : zero;
+            for (int j = 0; j < RT; j++) a[s][j] = A.h8(arow[j] + ka);
 #pragma unroll
             for (int m = 0; m < MT; m++) {
-                const bool on = in && live[m];
                 if constexpr (X16) {
-                    xh[s][m] = on ? *(const ad_h8 *)((const _Float16 *)x + xrow[m] + k) : zero;
+                    xh[s][m] = x.h8(xrow[m] + kx);
                 } else {
-                    const ad_f4 *p = (const ad_f4 *)((const float *)x + xrow[m] + k);
-                    xf[s][m][0] = on ? p[0] : (ad_f4){0, 0, 0, 0};
-                    xf[s][m][1] = on ? p[1] : (ad_f4){0, 0, 0, 0};
+                    xf[s][m][0] = x.f4(xrow[m] + kx);
+                    xf[s][m][1] = x.f4(xrow[m] + kx + 16);
                 }
             }
         }
 #pragma unroll
         for (int s = 0; s < DEP; s++) {
+            if (kb + 32 * s >= k1) break;
 #pragma unroll
             for (int j = 0; j < RT; j++) {
 #pragma unroll
@@ -156,31 +183,61 @@ __device__ __forceinline__ void ad_dots(const _Float16 *__restrict__ A, const vo
 // takes a second launch; reading it again from L2 per piece of n costs less.
 constexpr int kRowsThreads = 512;
 
-template <int RC>
-__device__ __forceinline__ void ad_up_rows(const AdapterJob &j, const float *h, int hs, int R, int rank, const _Float16 *B,
-                                           float scale, const size_t *yrow, int rows, int n0, int n1) {
-    for (int n = n0 + (int)threadIdx.x; n < n1; n += kRowsThreads) {
+// A thread's B rows for NP neighbouring passes over n (n, n + kRowsThreads, ..).
+template <int RT, int NP>
+struct AdB {
+    ad_h8 v[NP][2 * RT];
+    __device__ __forceinline__ void load(const AdBuf &B, int R, int rank, int n, int n1) {
+#pragma unroll
+        for (int q = 0; q < NP; q++) {
+            const int at = n + q * kRowsThreads;
+            const uint32_t row = at < n1 ? at * rank * 2u : kOff;
+#pragma unroll
+            for (int c = 0; c < 2 * RT; c++) {
+                v[q][c] = B.h8(8 * c < R ? row + 16 * c : kOff);
+            }
+        }
+    }
+};
+
+// Outputs of `rows` rows (at most RC at a time) at the passes that bv holds.
+template <int RC, int RT, int NP>
+__device__ __forceinline__ void ad_up_rows(const AdapterJob &j, const AdBuf &yb, const AdBuf &ob, const float *h, int hs, int R,
+                                           const AdB<RT, NP> &bv, float scale, const uint32_t *rows_of, int rows, int n, int n1) {
+    float y[NP][RC];
+    uint32_t at[NP][RC];  // elements of the window
+#pragma unroll
+    for (int q = 0; q < NP; q++) {
+#pragma unroll
+        for (int c = 0; c < RC; c++) {
+            const int nn = n + q * kRowsThreads;
+            at[q][c] = nn < n1 && c < rows ? rows_of[c] * j.n + nn : kOff;
+            y[q][c] = j.y16 ? yb.h1(2 * at[q][c]) : yb.f1(4 * min(at[q][c], kOff / 2));
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < NP; q++) {
+        if (n - (int)threadIdx.x + q * kRowsThreads >= n1) break;
         float s[RC] = {};
-        for (int r = 0; r < R; r += 8) {
-            const ad_h8 b = *(const ad_h8 *)(B + (size_t)n * rank + r);
+#pragma unroll
+        for (int r8 = 0; r8 < 2 * RT; r8++) {
+            if (8 * r8 >= R) continue;
+            const bool part = 8 * r8 + 8 > R;
+            if constexpr (RT > 1) __builtin_amdgcn_sched_barrier(0);  // h's reads stay by their products: all at once they would spill
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = r + e < R ? (float)b[e] : 0.0f;
+                const float v = part && 8 * r8 + e >= R ? 0.0f : (float)bv.v[q][r8][e];
 #pragma unroll
-                for (int c = 0; c < RC; c++) s[c] += h[c * hs + r + e] * v;
+                for (int c = 0; c < RC; c++) s[c] += h[c * hs + 8 * r8 + e] * v;
             }
         }
 #pragma unroll
         for (int c = 0; c < RC; c++) {
-            if (c >= rows) break;
-            const size_t at = yrow[c] + n;
-            float z = ad_load(j.y, j.y16, at);
-            if (R) z += scale * s[c];
-            z = ad_epi(z, j.epi);
+            const float z = ad_epi(R ? y[q][c] + scale * s[c] : y[q][c], j.epi);
             if (j.o16)
-                ((_Float16 *)j.out)[at] = (_Float16)z;
+                ob.put((_Float16)z, 2 * at[q][c]);
             else
-                ((float *)j.out)[at] = z;
+                ob.put(z, 4 * min(at[q][c], kOff / 2));
         }
     }
 }
@@ -188,12 +245,14 @@ __device__ __forceinline__ void ad_up_rows(const AdapterJob &j, const float *h, 
 template <int RT, bool X16>
 __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
     constexpr int HS = 16 * RT + 4, RG = RT < 4 ? RT : 4;
+    constexpr int NP = RT == 1 ? 5 : RT == 2 ? 3 : 1;  // B rows held from the start
     __shared__ float red[8][16][16 * RG + 4];
     __shared__ __align__(16) float h[16 * HS];
-    __shared__ size_t yrow[16];
+    __shared__ uint32_t rows_of[16];
     const AdapterJob &j = J.j[blockIdx.z];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const int win = blockIdx.y, G = gridDim.x;
+    const AdBuf xb = ad_rows(J, j.x, j.k, X16, win), yb = ad_rows(J, j.y, j.n, j.y16, win), ob = ad_rows(J, j.out, j.n, j.o16, win);
     const AdWindow w = ad_window(J, win, j.out != j.y || j.epi != GE_STORE);
     if (w.groups == 0) return;
     const int C = max(1, min(G / w.groups, (j.n + 255) / 256));
@@ -205,23 +264,25 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
         const AdGroup grp = ad_group(w, gi);
         const int R = grp.R;
         const float scale = grp.scale;
-        const _Float16 *A = j.a + (size_t)max(grp.a, 0) * J.rank * j.k, *B = j.b + (size_t)max(grp.a, 0) * j.n * J.rank;
+        const AdBuf A(j.a + (size_t)max(grp.a, 0) * J.rank * j.k, (size_t)R * j.k * 2);
+        const AdBuf B(j.b + (size_t)max(grp.a, 0) * j.n * J.rank, (size_t)j.n * J.rank * 2);
+        AdB<RT, NP> bv;
+        bv.load(B, R, J.rank, n0 + threadIdx.x, n1);
         for (int p0 = 0; p0 < grp.cnt; p0 += 16) {
             const int rows = min(16, grp.cnt - p0);
-            const size_t row = (size_t)win * kWin + __shfl(grp.row, p0 + i);
-            const size_t xrow[1] = {row * j.k};
-            const bool live[1] = {i < rows};
-            __syncthreads();  // the tile before is done with h and yrow
-            if (wave == 0 && g == 0) yrow[i] = row * j.n;
+            const uint32_t row = __shfl(grp.row, p0 + i);
+            const uint32_t xrow[1] = {i < rows ? row * j.k * (X16 ? 2 : 4) : kOff};
+            __syncthreads();  // the tile before is done with h and rows_of
+            if (wave == 0 && g == 0) rows_of[i] = row;
             if (R) {
                 ad_f4 acc[1][RT] = {};
-                ad_dots<RT, 1, X16, (RT <= 2 ? 5 : RT <= 4 ? 2 : 1)>(A, j.x, xrow, live, R, j.k, wave * ks, min(j.k, (wave + 1) * ks), acc);
+                ad_dots<RT, 1, X16, (RT == 1 ? 10 : RT == 2 ? 6 : RT == 4 ? 4 : 2)>(A, xb, xrow, j.k, wave * ks, min(j.k, (wave + 1) * ks), acc);
 #pragma unroll
                 for (int q = 0; q < RT; q += RG) {
 #pragma unroll
                     for (int t = 0; t < RG; t++) *(ad_f4 *)&red[wave][i][16 * t + 4 * g] = acc[0][q + t];
                     __syncthreads();
-                    for (int v = threadIdx.x; v < 16 * 16 * RG; v += kRowsThreads) {
+                    for (int v = threadIdx.x; v < rows * 16 * RG; v += kRowsThreads) {
                         const int hr = v / (16 * RG), hc = v % (16 * RG);
                         float s = 0.0f;
 #pragma unroll
@@ -233,79 +294,88 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
             } else {
                 __syncthreads();
             }
-            if (rows == 1)
-                ad_up_rows<1>(j, h, HS, R, J.rank, B, scale, yrow, rows, n0, n1);
-            else if (rows <= 4)
-                ad_up_rows<4>(j, h, HS, R, J.rank, B, scale, yrow, rows, n0, n1);
-            else
-                ad_up_rows<16>(j, h, HS, R, J.rank, B, scale, yrow, rows, n0, n1);
+            for (int n = n0 + (int)threadIdx.x; n - (int)threadIdx.x < n1; n += NP * kRowsThreads) {
+                if (n - (int)threadIdx.x > n0 || p0 > 0) bv.load(B, R, J.rank, n, n1);
+                if (rows == 1)
+                    ad_up_rows<1, RT, NP>(j, yb, ob, h, HS, R, bv, scale, rows_of, rows, n, n1);
+                else
+                    for (int c = 0; c < rows; c += 4) ad_up_rows<4, RT, NP>(j, yb, ob, h + c * HS, HS, R, bv, scale, rows_of + c, rows - c, n, n1);
+            }
         }
     }
 }
 
 // ------------------------------------------------ many rows: two launches
 // h of a window's rows: 4 waves over a slice of k, their sums added in wave
-// order into slice q of the work area, h[q][t][r].  The slice count of a group
-// follows from the window's groups (ad_slices), so the second launch knows it.
-constexpr int kDownThreads = 256;
+// order into slice q of the work area, h[q][t][r].  A wave's part of k is at
+// most 160, which it loads at once.
+constexpr int kDownThreads = 256, kDownK = 640;
 
-__device__ __forceinline__ int ad_slices(int G, int groups, int k) { return max(1, min(G / max(groups, 1), (k + 511) / 512)); }
+// Steps of 32 k whose operands fit about 128 registers.
+constexpr int ad_depth(int RT, int MT, bool x16) {
+    const int d = 128 / (4 * RT + (x16 ? 4 : 8) * MT);
+    return d < 1 ? 1 : d > 5 ? 5 : d;
+}
 
 template <int RT, int MT, bool X16>
-__device__ __forceinline__ void ad_down_tiles(const AdapterJobs &J, const AdapterJob &j, const AdGroup &grp, int win, int p0, int R,
-                                              const _Float16 *A, int k0, int k1, float *hq, float (*red)[16][16 * (RT < 4 ? RT : 4) + 4]) {
+__device__ __forceinline__ void ad_down_tiles(const AdapterJobs &J, const AdapterJob &j, const AdGroup &grp, int win, int R,
+                                              const AdBuf &A, const AdBuf &x, int k0, int k1, float *hq, float (*red)[16][16 * (RT < 4 ? RT : 4) + 4]) {
     constexpr int RG = RT < 4 ? RT : 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    size_t xrow[MT];
-    bool live[MT];
+    uint32_t xrow[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        xrow[m] = ((size_t)win * kWin + __shfl(grp.row, p0 + 16 * m + i)) * j.k;
-        live[m] = p0 + 16 * m + i < grp.cnt;
+        const uint32_t row = __shfl(grp.row, 16 * m + i);
+        xrow[m] = 16 * m + i < grp.cnt ? row * j.k * (X16 ? 2 : 4) : kOff;
     }
     const int ks = ((k1 - k0 + 3) / 4 + 31) / 32 * 32;
     ad_f4 acc[MT][RT] = {};
-    ad_dots<RT, MT, X16, (RT * MT <= 4 ? 4 : RT * MT <= 8 ? 2 : 1)>(A, j.x, xrow, live, R, j.k, min(k1, k0 + wave * ks), min(k1, k0 + (wave + 1) * ks), acc);
+    ad_dots<RT, MT, X16, ad_depth(RT, MT, X16)>(A, x, xrow, j.k, min(k1, k0 + wave * ks), min(k1, k0 + (wave + 1) * ks), acc);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
+        if (16 * m >= grp.cnt) break;
 #pragma unroll
         for (int q = 0; q < RT; q += RG) {
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < RG; t++) *(ad_f4 *)&red[wave][i][16 * t + 4 * g] = acc[m][q + t];
             __syncthreads();
-            for (int v = threadIdx.x; v < 16 * 16 * RG; v += kDownThreads) {
-                const int hr = v / (16 * RG), hc = v % (16 * RG), p = p0 + 16 * m + hr, r = 16 * q + hc;
-                const int row = __shfl(grp.row, p & 63);  // every lane of the wave gets here: 256 divides 256 RG
-                if (p < grp.cnt && r < R) hq[((size_t)win * kWin + row) * J.rank + r] = (red[0][hr][hc] + red[1][hr][hc]) + (red[2][hr][hc] + red[3][hr][hc]);
+            // four neighbouring ranks a thread
+            for (int v = threadIdx.x; v < 16 * 4 * RG; v += kDownThreads) {
+                const int hr = v / (4 * RG), hc = 4 * (v % (4 * RG)), p = 16 * m + hr, r = 16 * q + hc;
+                ad_f4 s = {0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < 4; u++) s += *(const ad_f4 *)&red[u][hr][hc];
+                const int row = __builtin_amdgcn_ds_bpermute(4 * (p & 63), grp.row);
+                // the second launch reads whole eights of ranks
+                if (p < grp.cnt && r < (R + 7) / 8 * 8) *(ad_f4 *)&hq[((size_t)win * kWin + row) * J.rank + r] = s;
             }
         }
     }
 }
 
+// grid (slices x slots, windows, jobs): slot s takes the window's groups s, s + slots, ...
 template <int RT, bool X16>
-__global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J) {
+__global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, int slots) {
     constexpr int RG = RT < 4 ? RT : 4;
     __shared__ float red[4][16][16 * RG + 4];
     const AdapterJob &j = J.j[blockIdx.z];
-    const int win = blockIdx.y, G = gridDim.x;
+    const int win = blockIdx.y, q = blockIdx.x / slots, k0 = q * kDownK, k1 = min(j.k, k0 + kDownK);
+    if (k0 >= j.k) return;
     const AdWindow w = ad_window(J, win, false);
-    if (w.groups == 0) return;
-    const int Q = ad_slices(G, w.groups, j.k), q = blockIdx.x / w.groups;
-    if (q >= Q) return;
-    const int ks = ((j.k + Q - 1) / Q + 127) / 128 * 128, k0 = q * ks, k1 = min(j.k, k0 + ks);
     float *hq = j.h + (size_t)q * J.rows * J.rank;
-    for (int gi = blockIdx.x % w.groups; gi < w.groups; gi += G) {
+    const AdBuf x = ad_rows(J, j.x, j.k, X16, win);
+    for (int gi = blockIdx.x % slots; gi < w.groups; gi += slots) {
         const AdGroup grp = ad_group(w, gi);
         const int R = grp.R;
-        const _Float16 *A = j.a + (size_t)grp.a * J.rank * j.k;
         if (R == 0) continue;
+        const AdBuf A(j.a + (size_t)grp.a * J.rank * j.k, (size_t)R * j.k * 2);
         if (grp.cnt <= 16)
-            ad_down_tiles<RT, 1, X16>(J, j, grp, win, 0, R, A, k0, k1, hq, red);
+            ad_down_tiles<RT, 1, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red);
         else if (grp.cnt <= 32)
-            ad_down_tiles<RT, 2, X16>(J, j, grp, win, 0, R, A, k0, k1, hq, red);
+            ad_down_tiles<RT, 2, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red);
         else
-            ad_down_tiles<RT, 4, X16>(J, j, grp, win, 0, R, A, k0, k1, hq, red);
+            ad_down_tiles<RT, 4, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red);
     }
 }
 
@@ -318,39 +388,74 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J) {
 constexpr int kUpThreads = 256, kUpN = 128;
 
 template <int RU>  // 32-rank units
-__global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int G) {
+__global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J) {
     constexpr int HS = 32 * RU + 8;
     __shared__ __align__(16) _Float16 hi[kWin][HS], lo[kWin][HS];
     __shared__ float back[kWin];  // scale times the row's power of two
-    __shared__ int rowof[kWin];
     const AdapterJob &j = J.j[blockIdx.z];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const int win = blockIdx.y, n0 = blockIdx.x * kUpN;
     if (n0 >= j.n) return;
     const AdWindow w = ad_window(J, win, j.out != j.y || j.epi != GE_STORE);
-    const int Q = ad_slices(G, __popcll(w.leaders), j.k);
-    const ad_h8 zero = {};
+    const int Q = (j.k + kDownK - 1) / kDownK;
+    const AdBuf yb = ad_rows(J, j.y, j.n, j.y16, win), ob = ad_rows(J, j.out, j.n, j.o16, win);
     for (int gi = 0; gi < w.groups; gi++) {
         const AdGroup grp = ad_group(w, gi);
-        const int R = grp.R;
-        const float scale = grp.scale;
-        const _Float16 *B = j.b + (size_t)max(grp.a, 0) * j.n * J.rank;
-        __syncthreads();
-        if (threadIdx.x < kWin) rowof[threadIdx.x] = grp.row;
-        __syncthreads();
+        const int R = grp.R, tiles = (grp.cnt + 15) / 16;
+        const AdBuf B(j.b + (size_t)max(grp.a, 0) * j.n * J.rank, R ? (size_t)j.n * J.rank * 2 : 0);
+        // everything the block reads is asked for before the first wait: a
+        // wave's two neighbouring 16-n tiles of B and y (a 128-byte line of fp32 a row) ...
+        const int n = n0 + 32 * wave;
+        ad_h8 b[2][RU];
+        ad_f4 y[2][4];
+        uint32_t at[2][4];  // elements of the window
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int nb = n + 16 * t + i;
+#pragma unroll
+            for (int u = 0; u < RU; u++) {
+                const int r = 32 * u + 8 * g;
+                b[t][u] = B.h8(r < R && nb < j.n ? (nb * J.rank + r) * 2u : kOff);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            if (m >= tiles) break;
+            const uint32_t row = __shfl(grp.row, 16 * m + i);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int nn = n + 16 * t + 4 * g;
+                at[t][m] = 16 * m + i < grp.cnt && nn < j.n ? row * j.n + nn : kOff / 2;
+                if (j.y16) {
+                    const ad_h4 v = yb.h4(2 * at[t][m]);
+                    y[t][m] = (ad_f4){(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+                } else {
+                    y[t][m] = yb.f4(4 * at[t][m]);
+                }
+            }
+        }
+        // ... and the slices of h: four threads a row, eights of ranks each
+        if (gi) __syncthreads();
         if (R) {
-            const int p = threadIdx.x >> 2, c = threadIdx.x & 3;  // four threads a row, 8 RU ranks each
-            float v[8 * RU];
+            const int p = threadIdx.x >> 2, c = threadIdx.x & 3;
+            const uint32_t hsrc = __builtin_amdgcn_ds_bpermute(4 * p, grp.row);  // all lanes take part
+            const uint32_t hrow = p < grp.cnt ? hsrc * J.rank * 4u + 32 * c : kOff;
+            ad_f4 v[RU][2] = {};
+#pragma unroll 4
+            for (int q = 0; q < Q; q++) {
+                const AdBuf hb = ad_rows(J, j.h + (size_t)q * J.rows * J.rank, J.rank, 0, win);
+#pragma unroll
+                for (int u = 0; u < RU; u++) {
+                    const uint32_t o = 32 * u + 8 * c < R ? hrow + 128 * u : kOff;
+                    v[u][0] += hb.f4(o);
+                    v[u][1] += hb.f4(o + 16);
+                }
+            }
             float top = 0.0f;
-            const size_t at = ((size_t)win * kWin + rowof[p]) * J.rank;
 #pragma unroll
             for (int e = 0; e < 8 * RU; e++) {
-                const int r = (e >> 3) * 32 + c * 8 + (e & 7);
-                float s = 0.0f;
-                if (p < grp.cnt && r < R) {
-                    for (int q = 0; q < Q; q++) s += j.h[(size_t)q * J.rows * J.rank + at + r];
-                }
-                v[e] = s;
+                float &s = ((float *)v)[e];
+                if ((e >> 3) * 32 + c * 8 + (e & 7) >= R) s = 0.0f;
                 top = fabsf(s) < INFINITY ? fmaxf(top, fabsf(s)) : top;
             }
             top = fmaxf(top, __shfl_xor(top, 1));
@@ -359,73 +464,67 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int G)
             if (top > 0.0f) ex = max(ilogbf(top) - 9, -126);
             const float down = ldexpf(1.0f, -ex);
 #pragma unroll
-            for (int e = 0; e < 8 * RU; e++) {
-                const int r = (e >> 3) * 32 + c * 8 + (e & 7);
-                const float s = v[e] * down;
-                const _Float16 a = (_Float16)s;
-                hi[p][r] = a;
-                lo[p][r] = fabsf(s) < INFINITY ? (_Float16)(s - (float)a) : (_Float16)0.0f;
-            }
-            if (c == 0) back[p] = scale * ldexpf(1.0f, ex);
-        }
-        __syncthreads();
-        const int tiles = (grp.cnt + 15) / 16;
-        for (int nt = wave; nt < kUpN / 16; nt += kUpThreads / 64) {
-            const int n = n0 + 16 * nt;
-            if (n >= j.n) break;
-            ad_h8 b[RU];
-#pragma unroll
             for (int u = 0; u < RU; u++) {
-                const int r = 32 * u + 8 * g;
-                b[u] = r < R && n + i < j.n ? *(const ad_h8 *)(B + (size_t)(n + i) * J.rank + r) : zero;
+                ad_h8 a, z;
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (r + e >= R) b[u][e] = (_Float16)0.0f;
+                for (int e = 0; e < 8; e++) {
+                    const float s = ((const float *)v[u])[e] * down;
+                    a[e] = (_Float16)s;
+                    z[e] = fabsf(s) < INFINITY ? (_Float16)(s - (float)a[e]) : (_Float16)0.0f;
+                }
+                *(ad_h8 *)&hi[p][32 * u + 8 * c] = a;
+                *(ad_h8 *)&lo[p][32 * u + 8 * c] = z;
             }
-            for (int m = 0; m < tiles; m++) {
-                const int p = 16 * m + i, nn = n + 4 * g;
-                ad_f4 acc = {0, 0, 0, 0};
-                if (R) {
+            if (c == 0) back[p] = grp.scale * ldexpf(1.0f, ex);
+            __syncthreads();
+            if (R % 8) {  // what lies past the adapter's own rank
 #pragma unroll
-                    for (int u = 0; u < RU; u++) {
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u], *(const ad_h8 *)&lo[p][32 * u + 8 * g], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[u], *(const ad_h8 *)&hi[p][32 * u + 8 * g], acc, 0, 0, 0);
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int u = 0; u < RU; u++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (32 * u + 8 * g + e >= R) b[t][u][e] = (_Float16)0.0f;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            if (m >= tiles) break;
+            const int p = 16 * m + i;
+            ad_f4 acc[2] = {};
+            if (R) {
+#pragma unroll
+                for (int u = 0; u < RU; u++) {
+                    const ad_h8 l = *(const ad_h8 *)&lo[p][32 * u + 8 * g], a = *(const ad_h8 *)&hi[p][32 * u + 8 * g];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[t][u], l, acc[t], 0, 0, 0);
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[t][u], a, acc[t], 0, 0, 0);
                     }
                 }
-                if (p >= grp.cnt || nn >= j.n) continue;
-                const size_t at = ((size_t)win * kWin + rowof[p]) * j.n + nn;
-                float z[4];
-                if (j.y16) {
-                    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-                    const h4 y = *(const h4 *)((const _Float16 *)j.y + at);
-                    for (int e = 0; e < 4; e++) z[e] = (float)y[e];
-                } else {
-                    const ad_f4 y = *(const ad_f4 *)((const float *)j.y + at);
-                    for (int e = 0; e < 4; e++) z[e] = y[e];
-                }
-                for (int e = 0; e < 4; e++) z[e] = ad_epi(R ? z[e] + back[p] * acc[e] : z[e], j.epi);
-                if (j.o16) {
-                    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-                    h4 o;
-                    for (int e = 0; e < 4; e++) o[e] = (_Float16)z[e];
-                    *(h4 *)((_Float16 *)j.out + at) = o;
-                } else {
-                    *(ad_f4 *)((float *)j.out + at) = (ad_f4){z[0], z[1], z[2], z[3]};
-                }
+            }
+            const float k = R ? back[p] : 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                ad_f4 z = y[t][m];
+#pragma unroll
+                for (int e = 0; e < 4; e++) z[e] = ad_epi(R ? z[e] + k * acc[t][e] : z[e], j.epi);
+                if (j.o16)
+                    ob.put((ad_h4){(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]}, 2 * at[t][m]);
+                else
+                    ob.put(z, 4 * at[t][m]);
             }
         }
     }
 }
 
-// Blocks of a window in the first of the two launches: about 512 in all.
-static int down_blocks(uint64_t rows, uint64_t njobs) {
-    const uint64_t wins = (rows + kWin - 1) / kWin;
-    return (int)std::max<uint64_t>(1, std::min<uint64_t>(32, 512 / (wins * njobs)));
-}
+static uint64_t down_slices(uint64_t k) { return (k + kDownK - 1) / kDownK; }
 
-uint64_t adapter_work_words(const rsv_adapter_job *, uint64_t njobs, uint64_t rank, uint64_t rows) {
+uint64_t adapter_work_words(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows) {
     if (rows <= kWin) return 1;
-    return njobs * rank * rows * down_blocks(rows, njobs);
+    uint64_t n = 0;
+    for (uint64_t i = 0; i < njobs; i++) n += down_slices(jobs[i].k) * rank * rows;
+    return n;
 }
 
 template <int RT, bool X16>
@@ -433,8 +532,8 @@ static void rows_rt(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid) {
     hipLaunchKernelGGL((k_adapter_rows<RT, X16>), grid, dim3(kRowsThreads), 0, ctx->stream, J);
 }
 template <int RT, bool X16>
-static void down_rt(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid) {
-    hipLaunchKernelGGL((k_adapter_down<RT, X16>), grid, dim3(kDownThreads), 0, ctx->stream, J);
+static void down_rt(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid, int slots) {
+    hipLaunchKernelGGL((k_adapter_down<RT, X16>), grid, dim3(kDownThreads), 0, ctx->stream, J, slots);
 }
 #define AD_RT(f, x16, ...)                                      \
     do {                                                        \
@@ -446,11 +545,13 @@ static void down_rt(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid) {
 
 int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work) {
     const int wins = (J.rows + kWin - 1) / kWin;
-    const int G = down_blocks(J.rows, J.njob);
-    int nmax = 0;
+    int nmax = 0, qmax = 0;
     for (int i = 0; i < J.njob; i++) {
-        J.j[i].h = work + (size_t)i * J.rank * J.rows * G;
+        const int q = (int)down_slices(J.j[i].k);
+        J.j[i].h = work;
+        work += (size_t)q * J.rank * J.rows;
         nmax = std::max(nmax, J.j[i].n);
+        qmax = std::max(qmax, q);
     }
     // jobs of one x type go together (each launch's kernel takes one)
     for (int x16 = 0; x16 < 2; x16++) {
@@ -464,16 +565,18 @@ int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work) {
             if (x16) AD_RT(rows_rt, true, ctx, S, grid);
             else AD_RT(rows_rt, false, ctx, S, grid);
         } else {
-            const dim3 grid(G, wins, S.njob);
-            if (x16) AD_RT(down_rt, true, ctx, S, grid);
-            else AD_RT(down_rt, false, ctx, S, grid);
+            // two slots a window for the few adapters of packed prompts, more where there are few windows
+            const int slots = std::max(2, std::min(kWin, 512 / (wins * S.njob * qmax)));
+            const dim3 grid(qmax * slots, wins, S.njob);
+            if (x16) AD_RT(down_rt, true, ctx, S, grid, slots);
+            else AD_RT(down_rt, false, ctx, S, grid, slots);
         }
     }
     if (J.rows > kWin) {
         const dim3 grid((nmax + kUpN - 1) / kUpN, wins, J.njob);
-        if (J.rank <= 32) hipLaunchKernelGGL((k_adapter_up<1>), grid, dim3(kUpThreads), 0, ctx->stream, J, G);
-        else if (J.rank <= 64) hipLaunchKernelGGL((k_adapter_up<2>), grid, dim3(kUpThreads), 0, ctx->stream, J, G);
-        else hipLaunchKernelGGL((k_adapter_up<4>), grid, dim3(kUpThreads), 0, ctx->stream, J, G);
+        if (J.rank <= 32) hipLaunchKernelGGL((k_adapter_up<1>), grid, dim3(kUpThreads), 0, ctx->stream, J);
+        else if (J.rank <= 64) hipLaunchKernelGGL((k_adapter_up<2>), grid, dim3(kUpThreads), 0, ctx->stream, J);
+        else hipLaunchKernelGGL((k_adapter_up<4>), grid, dim3(kUpThreads), 0, ctx->stream, J);
     }
     RSV_HIP(hipGetLastError());
     return 0;

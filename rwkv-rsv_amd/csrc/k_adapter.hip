@@ -29,7 +29,7 @@ constexpr int kBare = -1;  // the group of a window's rows without an adapter
 // first rows, then (with `bare`) one of the rows that have none.
 struct AdWindow {
     uint32_t id;        // the lane's adapter,
-    int rank;           // its own rank
+    uint32_t rank;      // its own rank
     float scale;        // and its scale
     uint64_t same;      // lanes with this lane's adapter
     uint64_t leaders;   // the first lane of each adapter
@@ -52,11 +52,12 @@ __device__ __forceinline__ uint64_t ad_lane64(uint64_t v, int lane) {
 __device__ __forceinline__ AdWindow ad_window(const AdapterJobs &J, int win, bool bare) {
     const int lane = threadIdx.x & 63, t = win * kWin + lane;
     AdWindow w;
-    w.id = t < J.rows ? J.row_adapter[t] : 0xFFFFFFFFu;
-    const bool has = w.id < (uint32_t)J.n_adapter;
-    // one load behind the id's, together with each other
-    w.rank = has ? J.ranks ? (int)min(J.ranks[w.id], (uint32_t)J.rank) : J.rank : 0;
-    w.scale = has ? J.scale[w.id] : 0.0f;
+    w.id = J.row_adapter[min(t, J.rows - 1)];
+    const bool has = t < J.rows && w.id < (uint32_t)J.n_adapter;
+    // one load behind the id's, together with each other; waited for at their use
+    const uint32_t known = min(w.id, (uint32_t)J.n_adapter - 1);
+    w.rank = J.ranks ? J.ranks[known] : J.rank;
+    w.scale = J.scale[known];
     w.same = __ballot(has);
     w.none = __ballot(t < J.rows && !has);
     for (int b = 0; (J.n_adapter - 1) >> b; b++) {
@@ -68,7 +69,7 @@ __device__ __forceinline__ AdWindow ad_window(const AdapterJobs &J, int win, boo
     return w;
 }
 
-__device__ __forceinline__ AdGroup ad_group(const AdWindow &w, int g) {
+__device__ __forceinline__ AdGroup ad_group(const AdapterJobs &J, const AdWindow &w, int g) {
     const int lane = threadIdx.x & 63;
     const uint64_t below = (1ull << lane) - 1;
     AdGroup r;
@@ -80,7 +81,7 @@ __device__ __forceinline__ AdGroup ad_group(const AdWindow &w, int g) {
         const uint64_t me = __ballot((w.leaders >> lane & 1) && __popcll(w.leaders & below) == g);
         const int l = __ffsll((long long)me) - 1;
         r.a = __builtin_amdgcn_readlane((int)w.id, l);
-        r.R = __builtin_amdgcn_readlane(w.rank, l);
+        r.R = (int)min((uint32_t)__builtin_amdgcn_readlane((int)w.rank, l), (uint32_t)J.rank);
         r.scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w.scale), l));
         mask = ad_lane64(w.same, l);
     }
@@ -101,6 +102,7 @@ __device__ __forceinline__ float ad_epi(float z, int epi) {
 // window's rows, at most 2^30 bytes; kOff added to an offset below that, once
 // or twice, stays past every size.
 constexpr uint32_t kOff = 0x40000000u;
+constexpr int kNt = 2;  // non-temporal: outputs that stream past the caches (r/k/v of 4096 rows: 111 -> 83 us)
 struct AdBuf {
     __amdgpu_buffer_rsrc_t r;
     __device__ __forceinline__ AdBuf(const void *p, size_t bytes) : r(__builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, (int)bytes, 0x00020000)) {}
@@ -109,8 +111,8 @@ struct AdBuf {
     __device__ __forceinline__ ad_h4 h4(uint32_t at) const { return __builtin_bit_cast(ad_h4, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0)); }
     __device__ __forceinline__ float f1(uint32_t at) const { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0)); }
     __device__ __forceinline__ float h1(uint32_t at) const { return (float)__builtin_bit_cast(_Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0)); }
-    __device__ __forceinline__ void put(ad_f4 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ad_u4, v), r, at, 0, 0); }
-    __device__ __forceinline__ void put(ad_h4 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(ad_u2, v), r, at, 0, 0); }
+    __device__ __forceinline__ void put(ad_f4 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ad_u4, v), r, at, 0, kNt); }
+    __device__ __forceinline__ void put(ad_h4 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(ad_u2, v), r, at, 0, kNt); }
     __device__ __forceinline__ void put(float v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), r, at, 0, 0); }
     __device__ __forceinline__ void put(_Float16 v, uint32_t at) const { __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), r, at, 0, 0); }
 };
@@ -218,6 +220,7 @@ __device__ __forceinline__ void ad_up_rows(const AdapterJob &j, const AdBuf &yb,
 #pragma unroll
     for (int q = 0; q < NP; q++) {
         if (n - (int)threadIdx.x + q * kRowsThreads >= n1) break;
+        if constexpr (RC > 1) __builtin_amdgcn_sched_barrier(0);
         float s[RC] = {};
 #pragma unroll
         for (int r8 = 0; r8 < 2 * RT; r8++) {
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
     const int n0 = (int)(blockIdx.x / w.groups) * piece, n1 = min(j.n, n0 + piece);
     const int ks = ((j.k + 7) / 8 + 31) / 32 * 32;  // k of a wave
     for (int gi = blockIdx.x % w.groups; gi < w.groups; gi += G) {
-        const AdGroup grp = ad_group(w, gi);
+        const AdGroup grp = ad_group(J, w, gi);
         const int R = grp.R;
         const float scale = grp.scale;
         const AdBuf A(j.a + (size_t)max(grp.a, 0) * J.rank * j.k, (size_t)R * j.k * 2);
@@ -298,6 +301,8 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
                 if (n - (int)threadIdx.x > n0 || p0 > 0) bv.load(B, R, J.rank, n, n1);
                 if (rows == 1)
                     ad_up_rows<1, RT, NP>(j, yb, ob, h, HS, R, bv, scale, rows_of, rows, n, n1);
+                else if (rows == 2)
+                    ad_up_rows<2, RT, NP>(j, yb, ob, h, HS, R, bv, scale, rows_of, rows, n, n1);
                 else
                     for (int c = 0; c < rows; c += 4) ad_up_rows<4, RT, NP>(j, yb, ob, h + c * HS, HS, R, bv, scale, rows_of + c, rows - c, n, n1);
             }
@@ -308,8 +313,11 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
 // ------------------------------------------------ many rows: two launches
 // h of a window's rows: 4 waves over a slice of k, their sums added in wave
 // order into slice q of the work area, h[q][t][r].  A wave's part of k is at
-// most 160, which it loads at once.
-constexpr int kDownThreads = 256, kDownK = 640;
+// most 320, loaded in two batches; fewer and longer slices cost less than the
+// reading of more partial sums by the second launch (r/k/v of 4096 rows: 99,
+// 83, 77, 81 us at slices of 320, 640, 1280, 2560; 517 rows of k = 10240: 41,
+// 31, 25, 28).
+constexpr int kDownThreads = 256, kDownWaves = kDownThreads / 64, kDownK = 1280;
 
 // Steps of 32 k whose operands fit about 128 registers.
 constexpr int ad_depth(int RT, int MT, bool x16) {
@@ -328,7 +336,7 @@ __device__ __forceinline__ void ad_down_tiles(const AdapterJobs &J, const Adapte
         const uint32_t row = __shfl(grp.row, 16 * m + i);
         xrow[m] = 16 * m + i < grp.cnt ? row * j.k * (X16 ? 2 : 4) : kOff;
     }
-    const int ks = ((k1 - k0 + 3) / 4 + 31) / 32 * 32;
+    const int ks = ((k1 - k0 + kDownWaves - 1) / kDownWaves + 31) / 32 * 32;
     ad_f4 acc[MT][RT] = {};
     ad_dots<RT, MT, X16, ad_depth(RT, MT, X16)>(A, x, xrow, j.k, min(k1, k0 + wave * ks), min(k1, k0 + (wave + 1) * ks), acc);
 #pragma unroll
@@ -345,7 +353,7 @@ __device__ __forceinline__ void ad_down_tiles(const AdapterJobs &J, const Adapte
                 const int hr = v / (4 * RG), hc = 4 * (v % (4 * RG)), p = 16 * m + hr, r = 16 * q + hc;
                 ad_f4 s = {0, 0, 0, 0};
 #pragma unroll
-                for (int u = 0; u < 4; u++) s += *(const ad_f4 *)&red[u][hr][hc];
+                for (int u = 0; u < kDownWaves; u++) s += *(const ad_f4 *)&red[u][hr][hc];
                 const int row = __builtin_amdgcn_ds_bpermute(4 * (p & 63), grp.row);
                 // the second launch reads whole eights of ranks
                 if (p < grp.cnt && r < (R + 7) / 8 * 8) *(ad_f4 *)&hq[((size_t)win * kWin + row) * J.rank + r] = s;
@@ -354,19 +362,22 @@ __device__ __forceinline__ void ad_down_tiles(const AdapterJobs &J, const Adapte
     }
 }
 
-// grid (slices x slots, windows, jobs): slot s takes the window's groups s, s + slots, ...
+// grid (slices, windows, slots x jobs): slot s takes the window's groups s, s +
+// slots, ... (slots in the slowest dimension, so that the blocks that find no
+// group do not leave whole XCDs idle)
 template <int RT, bool X16>
 __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, int slots) {
     constexpr int RG = RT < 4 ? RT : 4;
-    __shared__ float red[4][16][16 * RG + 4];
-    const AdapterJob &j = J.j[blockIdx.z];
-    const int win = blockIdx.y, q = blockIdx.x / slots, k0 = q * kDownK, k1 = min(j.k, k0 + kDownK);
+    __shared__ float red[kDownWaves][16][16 * RG + 4];
+    const int slot = blockIdx.z / J.njob;
+    const AdapterJob &j = J.j[blockIdx.z % J.njob];
+    const int win = blockIdx.y, q = blockIdx.x, k0 = q * kDownK, k1 = min(j.k, k0 + kDownK);
     if (k0 >= j.k) return;
     const AdWindow w = ad_window(J, win, false);
     float *hq = j.h + (size_t)q * J.rows * J.rank;
     const AdBuf x = ad_rows(J, j.x, j.k, X16, win);
-    for (int gi = blockIdx.x % slots; gi < w.groups; gi += slots) {
-        const AdGroup grp = ad_group(w, gi);
+    for (int gi = slot; gi < w.groups; gi += slots) {
+        const AdGroup grp = ad_group(J, w, gi);
         const int R = grp.R;
         if (R == 0) continue;
         const AdBuf A(j.a + (size_t)grp.a * J.rank * j.k, (size_t)R * j.k * 2);
@@ -387,20 +398,21 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, in
 // of one row, 16-byte loads of y and stores of out.
 constexpr int kUpThreads = 256, kUpN = 128;
 
-template <int RU>  // 32-rank units
-__global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J) {
+template <int RU, bool ONE>  // 32-rank units; one block for all groups of a window
+__global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int slots) {
     constexpr int HS = 32 * RU + 8;
     __shared__ __align__(16) _Float16 hi[kWin][HS], lo[kWin][HS];
     __shared__ float back[kWin];  // scale times the row's power of two
-    const AdapterJob &j = J.j[blockIdx.z];
+    const int slot = ONE ? 0 : blockIdx.z / J.njob, step = ONE ? 1 : slots;
+    const AdapterJob &j = J.j[ONE ? blockIdx.z : blockIdx.z % J.njob];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const int win = blockIdx.y, n0 = blockIdx.x * kUpN;
     if (n0 >= j.n) return;
     const AdWindow w = ad_window(J, win, j.out != j.y || j.epi != GE_STORE);
     const int Q = (j.k + kDownK - 1) / kDownK;
     const AdBuf yb = ad_rows(J, j.y, j.n, j.y16, win), ob = ad_rows(J, j.out, j.n, j.o16, win);
-    for (int gi = 0; gi < w.groups; gi++) {
-        const AdGroup grp = ad_group(w, gi);
+    for (int gi = slot; gi < w.groups; gi += step) {
+        const AdGroup grp = ad_group(J, w, gi);
         const int R = grp.R, tiles = (grp.cnt + 15) / 16;
         const AdBuf B(j.b + (size_t)max(grp.a, 0) * j.n * J.rank, R ? (size_t)j.n * J.rank * 2 : 0);
         // everything the block reads is asked for before the first wait: a
@@ -435,13 +447,13 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J) {
             }
         }
         // ... and the slices of h: four threads a row, eights of ranks each
-        if (gi) __syncthreads();
+        if (gi != slot) __syncthreads();
         if (R) {
             const int p = threadIdx.x >> 2, c = threadIdx.x & 3;
             const uint32_t hsrc = __builtin_amdgcn_ds_bpermute(4 * p, grp.row);  // all lanes take part
             const uint32_t hrow = p < grp.cnt ? hsrc * J.rank * 4u + 32 * c : kOff;
             ad_f4 v[RU][2] = {};
-#pragma unroll 4
+#pragma unroll 8
             for (int q = 0; q < Q; q++) {
                 const AdBuf hb = ad_rows(J, j.h + (size_t)q * J.rows * J.rank, J.rank, 0, win);
 #pragma unroll
@@ -460,9 +472,9 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J) {
             }
             top = fmaxf(top, __shfl_xor(top, 1));
             top = fmaxf(top, __shfl_xor(top, 2));
-            int ex = 0;
-            if (top > 0.0f) ex = max(ilogbf(top) - 9, -126);
-            const float down = ldexpf(1.0f, -ex);
+            // the row's power of two from its exponent bits: 2^ex with top / 2^ex in [2^9, 2^10)
+            const int ex = max((int)(__float_as_uint(top) >> 23) - 127 - 9, -126);
+            const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
 #pragma unroll
             for (int u = 0; u < RU; u++) {
                 ad_h8 a, z;
@@ -475,7 +487,7 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J) {
                 *(ad_h8 *)&hi[p][32 * u + 8 * c] = a;
                 *(ad_h8 *)&lo[p][32 * u + 8 * c] = z;
             }
-            if (c == 0) back[p] = grp.scale * ldexpf(1.0f, ex);
+            if (c == 0) back[p] = grp.scale * __uint_as_float((uint32_t)(127 + ex) << 23);
             __syncthreads();
             if (R % 8) {  // what lies past the adapter's own rank
 #pragma unroll
@@ -535,6 +547,13 @@ template <int RT, bool X16>
 static void down_rt(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid, int slots) {
     hipLaunchKernelGGL((k_adapter_down<RT, X16>), grid, dim3(kDownThreads), 0, ctx->stream, J, slots);
 }
+template <int RU>
+static void up_ru(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid, int slots) {
+    if (slots == 1)
+        hipLaunchKernelGGL((k_adapter_up<RU, true>), grid, dim3(kUpThreads), 0, ctx->stream, J, 1);
+    else
+        hipLaunchKernelGGL((k_adapter_up<RU, false>), grid, dim3(kUpThreads), 0, ctx->stream, J, slots);
+}
 #define AD_RT(f, x16, ...)                                      \
     do {                                                        \
         if (J.rank <= 16) f<1, x16>(__VA_ARGS__);               \
@@ -565,18 +584,20 @@ int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work) {
             if (x16) AD_RT(rows_rt, true, ctx, S, grid);
             else AD_RT(rows_rt, false, ctx, S, grid);
         } else {
-            // two slots a window for the few adapters of packed prompts, more where there are few windows
-            const int slots = std::max(2, std::min(kWin, 512 / (wins * S.njob * qmax)));
-            const dim3 grid(qmax * slots, wins, S.njob);
+            // slots a window: about 512 blocks in all
+            const int slots = std::max(1, std::min(kWin, 512 / (wins * S.njob * qmax)));
+            const dim3 grid(qmax, wins, slots * S.njob);
             if (x16) AD_RT(down_rt, true, ctx, S, grid, slots);
             else AD_RT(down_rt, false, ctx, S, grid, slots);
         }
     }
     if (J.rows > kWin) {
-        const dim3 grid((nmax + kUpN - 1) / kUpN, wins, J.njob);
-        if (J.rank <= 32) hipLaunchKernelGGL((k_adapter_up<1>), grid, dim3(kUpThreads), 0, ctx->stream, J);
-        else if (J.rank <= 64) hipLaunchKernelGGL((k_adapter_up<2>), grid, dim3(kUpThreads), 0, ctx->stream, J);
-        else hipLaunchKernelGGL((k_adapter_up<4>), grid, dim3(kUpThreads), 0, ctx->stream, J);
+        const int chunks = (nmax + kUpN - 1) / kUpN;
+        const int slots = std::max(1, std::min(kWin, 1024 / (chunks * wins * J.njob)));
+        const dim3 grid(chunks, wins, slots * J.njob);
+        if (J.rank <= 32) up_ru<1>(ctx, J, grid, slots);
+        else if (J.rank <= 64) up_ru<2>(ctx, J, grid, slots);
+        else up_ru<4>(ctx, J, grid, slots);
     }
     RSV_HIP(hipGetLastError());
     return 0;

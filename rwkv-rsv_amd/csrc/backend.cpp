@@ -1832,7 +1832,7 @@ extern "C" int rsv_adapter_multi(rsv_ctx *ctx, const rsv_adapter_job *jobs, uint
         if (clash || work == row_adapter || work == scale || work == ranks)
             return RSV_FAIL("adapter_multi job %llu: out or work is another operand of the call (out may be its own y)", (unsigned long long)i);
     }
-    return launch_adapter(ctx, J, F32P(wk));
+    return launch_adapter(ctx, J, jobs, F32P(wk));
 }
 
 static int logits_limits(uint64_t n, uint64_t rows, const char *what) {

@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
 // reading of more partial sums by the second launch (r/k/v of 4096 rows: 99,
 // 83, 77, 81 us at slices of 320, 640, 1280, 2560; 517 rows of k = 10240: 41,
 // 31, 25, 28).
-constexpr int kDownThreads = 256, kDownWaves = kDownThreads / 64, kDownK = 1280;
+constexpr int kDownThreads = 256, kDownWaves = kDownThreads / 64;
 
 // Steps of 32 k whose operands fit about 128 registers.
 constexpr int ad_depth(int RT, int MT, bool x16) {
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, in
     __shared__ float red[kDownWaves][16][16 * RG + 4];
     const int slot = blockIdx.z / J.njob;
     const AdapterJob &j = J.j[blockIdx.z % J.njob];
-    const int win = blockIdx.y, q = blockIdx.x, k0 = q * kDownK, k1 = min(j.k, k0 + kDownK);
+    const int win = blockIdx.y, q = blockIdx.x, k0 = q * J.slice, k1 = min(j.k, k0 + J.slice);
     if (k0 >= j.k) return;
     const AdWindow w = ad_window(J, win, false);
     float *hq = j.h + (size_t)q * J.rows * J.rank;
@@ -398,6 +398,76 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, in
 // of one row, 16-byte loads of y and stores of out.
 constexpr int kUpThreads = 256, kUpN = 128;
 
+// h of row p of a group into hi, lo and back: four lanes a row (c), eights of
+// ranks each.  src: the window row; live: the row is the group's.
+template <int RU>
+__device__ __forceinline__ void ad_stage(const AdapterJobs &J, const AdapterJob &j, int win, int Q, int R, float scale, int p, int c,
+                                         uint32_t src, bool live, _Float16 (*hi)[32 * RU + 8], _Float16 (*lo)[32 * RU + 8], float *back) {
+    const uint32_t hrow = live ? src * J.rank * 4u + 32 * c : kOff;
+    ad_f4 v[RU][2] = {};
+#pragma unroll 8
+    for (int q = 0; q < Q; q++) {
+        const AdBuf hb = ad_rows(J, j.h + (size_t)q * J.rows * J.rank, J.rank, 0, win);
+#pragma unroll
+        for (int u = 0; u < RU; u++) {
+            const uint32_t o = 32 * u + 8 * c < R ? hrow + 128 * u : kOff;
+            v[u][0] += hb.f4(o);
+            v[u][1] += hb.f4(o + 16);
+        }
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8 * RU; e++) {
+        float &s = ((float *)v)[e];
+        if ((e >> 3) * 32 + c * 8 + (e & 7) >= R) s = 0.0f;
+        top = fabsf(s) < INFINITY ? fmaxf(top, fabsf(s)) : top;
+    }
+    top = fmaxf(top, __shfl_xor(top, 1));
+    top = fmaxf(top, __shfl_xor(top, 2));
+    // the row's power of two from its exponent bits: 2^ex with top / 2^ex in [2^9, 2^10)
+    const int ex = max((int)(__float_as_uint(top) >> 23) - 127 - 9, -126);
+    const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+    for (int u = 0; u < RU; u++) {
+        ad_h8 a, z;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float s = ((const float *)v[u])[e] * down;
+            a[e] = (_Float16)s;
+            z[e] = fabsf(s) < INFINITY ? (_Float16)(s - (float)a[e]) : (_Float16)0.0f;
+        }
+        *(ad_h8 *)&hi[p][32 * u + 8 * c] = a;
+        *(ad_h8 *)&lo[p][32 * u + 8 * c] = z;
+    }
+    if (c == 0) back[p] = scale * __uint_as_float((uint32_t)(127 + ex) << 23);
+}
+
+// Four neighbouring n of a row of y (elements at `at` of the window), and the outputs.
+__device__ __forceinline__ ad_f4 ad_y4(const AdapterJob &j, const AdBuf &yb, uint32_t at) {
+    if (j.y16) {
+        const ad_h4 v = yb.h4(2 * at);
+        return (ad_f4){(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+    }
+    return yb.f4(4 * at);
+}
+__device__ __forceinline__ void ad_out4(const AdapterJob &j, const AdBuf &ob, ad_f4 z, uint32_t at) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) z[e] = ad_epi(z[e], j.epi);
+    if (j.o16)
+        ob.put((ad_h4){(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]}, 2 * at);
+    else
+        ob.put(z, 4 * at);
+}
+template <int RU>
+__device__ __forceinline__ void ad_clear_past(ad_h8 (&b)[RU], int R, int g) {  // what lies past the adapter's own rank
+    if (R % 8 == 0) return;
+#pragma unroll
+    for (int u = 0; u < RU; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (32 * u + 8 * g + e >= R) b[u][e] = (_Float16)0.0f;
+}
+
 template <int RU, bool ONE>  // 32-rank units; one block for all groups of a window
 __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int slots) {
     constexpr int HS = 32 * RU + 8;
@@ -409,7 +479,7 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int sl
     const int win = blockIdx.y, n0 = blockIdx.x * kUpN;
     if (n0 >= j.n) return;
     const AdWindow w = ad_window(J, win, j.out != j.y || j.epi != GE_STORE);
-    const int Q = (j.k + kDownK - 1) / kDownK;
+    const int Q = (j.k + J.slice - 1) / J.slice;
     const AdBuf yb = ad_rows(J, j.y, j.n, j.y16, win), ob = ad_rows(J, j.out, j.n, j.o16, win);
     for (int gi = slot; gi < w.groups; gi += step) {
         const AdGroup grp = ad_group(J, w, gi);
@@ -438,66 +508,18 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int sl
             for (int t = 0; t < 2; t++) {
                 const int nn = n + 16 * t + 4 * g;
                 at[t][m] = 16 * m + i < grp.cnt && nn < j.n ? row * j.n + nn : kOff / 2;
-                if (j.y16) {
-                    const ad_h4 v = yb.h4(2 * at[t][m]);
-                    y[t][m] = (ad_f4){(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-                } else {
-                    y[t][m] = yb.f4(4 * at[t][m]);
-                }
+                y[t][m] = ad_y4(j, yb, at[t][m]);
             }
         }
         // ... and the slices of h: four threads a row, eights of ranks each
         if (gi != slot) __syncthreads();
         if (R) {
-            const int p = threadIdx.x >> 2, c = threadIdx.x & 3;
-            const uint32_t hsrc = __builtin_amdgcn_ds_bpermute(4 * p, grp.row);  // all lanes take part
-            const uint32_t hrow = p < grp.cnt ? hsrc * J.rank * 4u + 32 * c : kOff;
-            ad_f4 v[RU][2] = {};
-#pragma unroll 8
-            for (int q = 0; q < Q; q++) {
-                const AdBuf hb = ad_rows(J, j.h + (size_t)q * J.rows * J.rank, J.rank, 0, win);
-#pragma unroll
-                for (int u = 0; u < RU; u++) {
-                    const uint32_t o = 32 * u + 8 * c < R ? hrow + 128 * u : kOff;
-                    v[u][0] += hb.f4(o);
-                    v[u][1] += hb.f4(o + 16);
-                }
-            }
-            float top = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8 * RU; e++) {
-                float &s = ((float *)v)[e];
-                if ((e >> 3) * 32 + c * 8 + (e & 7) >= R) s = 0.0f;
-                top = fabsf(s) < INFINITY ? fmaxf(top, fabsf(s)) : top;
-            }
-            top = fmaxf(top, __shfl_xor(top, 1));
-            top = fmaxf(top, __shfl_xor(top, 2));
-            // the row's power of two from its exponent bits: 2^ex with top / 2^ex in [2^9, 2^10)
-            const int ex = max((int)(__float_as_uint(top) >> 23) - 127 - 9, -126);
-            const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-#pragma unroll
-            for (int u = 0; u < RU; u++) {
-                ad_h8 a, z;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float s = ((const float *)v[u])[e] * down;
-                    a[e] = (_Float16)s;
-                    z[e] = fabsf(s) < INFINITY ? (_Float16)(s - (float)a[e]) : (_Float16)0.0f;
-                }
-                *(ad_h8 *)&hi[p][32 * u + 8 * c] = a;
-                *(ad_h8 *)&lo[p][32 * u + 8 * c] = z;
-            }
-            if (c == 0) back[p] = grp.scale * __uint_as_float((uint32_t)(127 + ex) << 23);
+            const int p = threadIdx.x >> 2;
+            const uint32_t src = __builtin_amdgcn_ds_bpermute(4 * p, grp.row);  // all lanes take part
+            ad_stage<RU>(J, j, win, Q, R, grp.scale, p, threadIdx.x & 3, src, p < grp.cnt, hi, lo, back);
             __syncthreads();
-            if (R % 8) {  // what lies past the adapter's own rank
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int u = 0; u < RU; u++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (32 * u + 8 * g + e >= R) b[t][u][e] = (_Float16)0.0f;
-            }
+            ad_clear_past(b[0], R, g);
+            ad_clear_past(b[1], R, g);
         }
 #pragma unroll
         for (int m = 0; m < 4; m++) {
@@ -518,24 +540,26 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int sl
             const float k = R ? back[p] : 0.0f;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                ad_f4 z = y[t][m];
-#pragma unroll
-                for (int e = 0; e < 4; e++) z[e] = ad_epi(R ? z[e] + k * acc[t][e] : z[e], j.epi);
-                if (j.o16)
-                    ob.put((ad_h4){(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]}, 2 * at[t][m]);
-                else
-                    ob.put(z, 4 * at[t][m]);
+                ad_out4(j, ob, R ? y[t][m] + k * acc[t] : y[t][m], at[t][m]);
             }
         }
     }
 }
 
-static uint64_t down_slices(uint64_t k) { return (k + kDownK - 1) / kDownK; }
+// k of a slice in the first of the two launches: long slices leave the second
+// launch fewer partial sums to read, but a launch that would leave most of the
+// chip idle is over sooner with short ones.
+static uint64_t down_slice(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rows) {
+    uint64_t blocks = 0;
+    for (uint64_t i = 0; i < njobs; i++) blocks += (rows + kWin - 1) / kWin * ((jobs[i].k + 1279) / 1280);
+    return blocks <= 32 ? 640 : 1280;
+}
 
 uint64_t adapter_work_words(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows) {
     if (rows <= kWin) return 1;
+    const uint64_t slice = down_slice(jobs, njobs, rows);
     uint64_t n = 0;
-    for (uint64_t i = 0; i < njobs; i++) n += down_slices(jobs[i].k) * rank * rows;
+    for (uint64_t i = 0; i < njobs; i++) n += (jobs[i].k + slice - 1) / slice * rank * rows;
     return n;
 }
 
@@ -562,11 +586,12 @@ static void up_ru(rsv_ctx *ctx, const AdapterJobs &J, dim3 grid, int slots) {
         else f<8, x16>(__VA_ARGS__);                            \
     } while (0)
 
-int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work) {
+int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, const rsv_adapter_job *jobs, float *work) {
     const int wins = (J.rows + kWin - 1) / kWin;
+    J.slice = (int)down_slice(jobs, J.njob, J.rows);
     int nmax = 0, qmax = 0;
     for (int i = 0; i < J.njob; i++) {
-        const int q = (int)down_slices(J.j[i].k);
+        const int q = (J.j[i].k + J.slice - 1) / J.slice;
         J.j[i].h = work;
         work += (size_t)q * J.rank * J.rows;
         nmax = std::max(nmax, J.j[i].n);
@@ -584,8 +609,9 @@ int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work) {
             if (x16) AD_RT(rows_rt, true, ctx, S, grid);
             else AD_RT(rows_rt, false, ctx, S, grid);
         } else {
-            // slots a window: about 512 blocks in all
-            const int slots = std::max(1, std::min(kWin, 512 / (wins * S.njob * qmax)));
+            // slots a window: about 512 blocks in all, and two where a packed chunk has
+            // windows with the end of one request and the start of the next (75 -> 70 us at 4096 rows)
+            const int slots = std::max(2, std::min(kWin, 512 / (wins * S.njob * qmax)));
             const dim3 grid(qmax, wins, slots * S.njob);
             if (x16) AD_RT(down_rt, true, ctx, S, grid, slots);
             else AD_RT(down_rt, false, ctx, S, grid, slots);

@@ -315,10 +315,10 @@ struct AdapterJobs {
     AdapterJob j[kMaxJobs];
     const uint32_t *row_adapter, *ranks;  // [rows]; [n_adapter] or null
     const float *scale;                   // [n_adapter]
-    int njob, n_adapter, rank, rows;
+    int njob, n_adapter, rank, rows, slice;  // slice: k of a partial sum (filled by the launcher)
 };
 uint64_t adapter_work_words(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows);
-int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, float *work);
+int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, const rsv_adapter_job *jobs, float *work);
 // Draws and log-probabilities from logits rows (k_logits.hip).
 constexpr uint64_t kLogitsMaxN = (uint64_t)1 << 20;
 uint64_t logits_work_words(uint64_t n, uint64_t rows);

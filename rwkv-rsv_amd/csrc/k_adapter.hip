@@ -319,26 +319,87 @@ __global__ __launch_bounds__(kRowsThreads) void k_adapter_rows(AdapterJobs J) {
 // 31, 25, 28).
 constexpr int kDownThreads = 256, kDownWaves = kDownThreads / 64;
 
-// Steps of 32 k whose operands fit about 128 registers.
-constexpr int ad_depth(int RT, int MT, bool x16) {
-    const int d = 128 / (4 * RT + (x16 ? 4 : 8) * MT);
-    return d < 1 ? 1 : d > 5 ? 5 : d;
+// Lines of 128 bytes a row (64 k of fp16, 32 of fp32) whose operands fit about 128 registers.
+constexpr int ad_lines(int RT, int MT, bool x16) {
+    const int d = 128 / (8 * MT + (x16 ? 8 : 4) * RT);
+    return d < 1 ? 1 : d > 3 ? 3 : d;
+}
+
+// ad_dots for whole windows: x comes as eight lanes a row, whole lines, and
+// through LDS (a wave's own 16 x 128 bytes) into the operands' layout.  rows:
+// byte offsets of rows l/8 and 8 + l/8 of each tile.
+template <int RT, int MT, bool X16, int NL>
+__device__ __forceinline__ void ad_dots_lines(const AdBuf &A, const AdBuf &x, const uint32_t (&rows)[MT][2], int K, int k0, int k1,
+                                              ad_f4 (&acc)[MT][RT], float (*tile)[36]) {
+    constexpr int LK = X16 ? 64 : 32, ST = LK / 32;  // k of a line, its steps of 32
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    uint32_t arow[RT];
+#pragma unroll
+    for (int j = 0; j < RT; j++) arow[j] = (16 * j + i) * K * 2u;
+    for (int kb = k0; kb < k1; kb += LK * NL) {
+        ad_h8 a[NL][ST][RT];
+        ad_f4 q[NL][MT][2];
+#pragma unroll
+        for (int l = 0; l < NL; l++) {
+            if (kb + LK * l >= k1) break;
+            const uint32_t kx = kb + LK * l + (lane & 7) * (X16 ? 8 : 4), ox = (int)kx < k1 ? kx * (X16 ? 2 : 4) : 2 * kOff;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                q[l][m][0] = x.f4(rows[m][0] + ox);
+                q[l][m][1] = x.f4(rows[m][1] + ox);
+            }
+#pragma unroll
+            for (int s = 0; s < ST; s++) {
+                const uint32_t k = kb + LK * l + 32 * s + 8 * g, oa = (int)k < k1 ? 2 * k : 2 * kOff;
+#pragma unroll
+                for (int j = 0; j < RT; j++) a[l][s][j] = A.h8(arow[j] + oa);
+            }
+        }
+#pragma unroll
+        for (int l = 0; l < NL; l++) {
+            if (kb + LK * l >= k1) break;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                *(ad_f4 *)&tile[lane >> 3][4 * (lane & 7)] = q[l][m][0];
+                *(ad_f4 *)&tile[8 + (lane >> 3)][4 * (lane & 7)] = q[l][m][1];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                const ad_f4 x0 = *(const ad_f4 *)&tile[i][X16 ? 4 * g : 8 * g], x1 = *(const ad_f4 *)&tile[i][X16 ? 16 + 4 * g : 8 * g + 4];
+#pragma unroll
+                for (int j = 0; j < RT; j++) {
+                    if constexpr (X16) {
+                        acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[l][0][j], __builtin_bit_cast(ad_h8, x0), acc[m][j], 0, 0, 0);
+                        acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[l][ST - 1][j], __builtin_bit_cast(ad_h8, x1), acc[m][j], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)a[l][0][j][e], e < 4 ? x0[e & 3] : x1[e & 3], acc[m][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
 }
 
 template <int RT, int MT, bool X16>
 __device__ __forceinline__ void ad_down_tiles(const AdapterJobs &J, const AdapterJob &j, const AdGroup &grp, int win, int R,
-                                              const AdBuf &A, const AdBuf &x, int k0, int k1, float *hq, float (*red)[16][16 * (RT < 4 ? RT : 4) + 4]) {
+                                              const AdBuf &A, const AdBuf &x, int k0, int k1, float *hq, float (*red)[16][16 * (RT < 4 ? RT : 4) + 4],
+                                              float (*tile)[16][36]) {
     constexpr int RG = RT < 4 ? RT : 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    uint32_t xrow[MT];
+    uint32_t rows[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        const uint32_t row = __shfl(grp.row, 16 * m + i);
-        xrow[m] = 16 * m + i < grp.cnt ? row * j.k * (X16 ? 2 : 4) : kOff;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int p = 16 * m + 8 * h + (lane >> 3);
+            const uint32_t row = __shfl(grp.row, p);
+            rows[m][h] = p < grp.cnt ? row * j.k * (X16 ? 2 : 4) : kOff;
+        }
     }
-    const int ks = ((k1 - k0 + kDownWaves - 1) / kDownWaves + 31) / 32 * 32;
+    const int ks = ((k1 - k0 + kDownWaves - 1) / kDownWaves + 63) / 64 * 64;
     ad_f4 acc[MT][RT] = {};
-    ad_dots<RT, MT, X16, ad_depth(RT, MT, X16)>(A, x, xrow, j.k, min(k1, k0 + wave * ks), min(k1, k0 + (wave + 1) * ks), acc);
+    ad_dots_lines<RT, MT, X16, ad_lines(RT, MT, X16)>(A, x, rows, j.k, min(k1, k0 + wave * ks), min(k1, k0 + (wave + 1) * ks), acc, tile[wave]);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         if (16 * m >= grp.cnt) break;
@@ -369,6 +430,7 @@ template <int RT, bool X16>
 __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, int slots) {
     constexpr int RG = RT < 4 ? RT : 4;
     __shared__ float red[kDownWaves][16][16 * RG + 4];
+    __shared__ __align__(16) float tile[kDownWaves][16][36];
     const int slot = blockIdx.z / J.njob;
     const AdapterJob &j = J.j[blockIdx.z % J.njob];
     const int win = blockIdx.y, q = blockIdx.x, k0 = q * J.slice, k1 = min(j.k, k0 + J.slice);
@@ -382,11 +444,11 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, in
         if (R == 0) continue;
         const AdBuf A(j.a + (size_t)grp.a * J.rank * j.k, (size_t)R * j.k * 2);
         if (grp.cnt <= 16)
-            ad_down_tiles<RT, 1, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red);
+            ad_down_tiles<RT, 1, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red, tile);
         else if (grp.cnt <= 32)
-            ad_down_tiles<RT, 2, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red);
+            ad_down_tiles<RT, 2, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red, tile);
         else
-            ad_down_tiles<RT, 4, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red);
+            ad_down_tiles<RT, 4, X16>(J, j, grp, win, R, A, x, k0, k1, hq, red, tile);
     }
 }
 
@@ -395,7 +457,7 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, in
 // a power of two to [2^9, 2^10): 22 bits of every element that counts in its
 // row's sum, so the products run on v_mfma_f32_16x16x32_f16 with fp32's
 // accuracy.  B's rows are the left operand: a lane holds four neighbouring n
-// of one row, 16-byte loads of y and stores of out.
+// of one row.
 constexpr int kUpThreads = 256, kUpN = 128;
 
 // h of row p of a group into hi, lo and back: four lanes a row (c), eights of
@@ -469,10 +531,11 @@ __device__ __forceinline__ void ad_clear_past(ad_h8 (&b)[RU], int R, int g) {  /
 }
 
 template <int RU, bool ONE>  // 32-rank units; one block for all groups of a window
-__global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int slots) {
+__global__ __launch_bounds__(kUpThreads, RU <= 2 ? 4 : 2) void k_adapter_up(AdapterJobs J, int slots) {
     constexpr int HS = 32 * RU + 8;
     __shared__ __align__(16) _Float16 hi[kWin][HS], lo[kWin][HS];
     __shared__ float back[kWin];  // scale times the row's power of two
+    __shared__ __align__(16) float tile[kUpThreads / 64][16][36];
     const int slot = ONE ? 0 : blockIdx.z / J.njob, step = ONE ? 1 : slots;
     const AdapterJob &j = J.j[ONE ? blockIdx.z : blockIdx.z % J.njob];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -486,11 +549,13 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int sl
         const int R = grp.R, tiles = (grp.cnt + 15) / 16;
         const AdBuf B(j.b + (size_t)max(grp.a, 0) * j.n * J.rank, R ? (size_t)j.n * J.rank * 2 : 0);
         // everything the block reads is asked for before the first wait: a
-        // wave's two neighbouring 16-n tiles of B and y (a 128-byte line of fp32 a row) ...
-        const int n = n0 + 32 * wave;
+        // wave's two neighbouring 16-n tiles of B, its 32 n of y as eight lanes
+        // a row (a whole 128-byte line of fp32: 64 bytes a row at a time took
+        // 71 us for r/k/v of 4096 rows, this 55) ...
+        const int n = n0 + 32 * wave, yn = n + 4 * (lane & 7), yrow = lane >> 3;
         ad_h8 b[2][RU];
-        ad_f4 y[2][4];
-        uint32_t at[2][4];  // elements of the window
+        ad_f4 y[4][2];
+        uint32_t at[4][2];  // elements of the window
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const int nb = n + 16 * t + i;
@@ -503,12 +568,12 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int sl
 #pragma unroll
         for (int m = 0; m < 4; m++) {
             if (m >= tiles) break;
-            const uint32_t row = __shfl(grp.row, 16 * m + i);
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const int nn = n + 16 * t + 4 * g;
-                at[t][m] = 16 * m + i < grp.cnt && nn < j.n ? row * j.n + nn : kOff / 2;
-                y[t][m] = ad_y4(j, yb, at[t][m]);
+                const int p = 16 * m + 8 * t + yrow;
+                const uint32_t row = __shfl(grp.row, p);
+                at[m][t] = p < grp.cnt && yn < j.n ? row * j.n + yn : kOff / 2;
+                y[m][t] = ad_y4(j, yb, at[m][t]);
             }
         }
         // ... and the slices of h: four threads a row, eights of ranks each
@@ -537,10 +602,18 @@ __global__ __launch_bounds__(kUpThreads) void k_adapter_up(AdapterJobs J, int sl
                     }
                 }
             }
-            const float k = R ? back[p] : 0.0f;
+            // the tile through LDS: from (row, 4 n) of 16 rows to eight lanes a row
+            if (R) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int t = 0; t < 2; t++) *(ad_f4 *)&tile[wave][i][16 * t + 4 * g] = back[p] * acc[t];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                ad_out4(j, ob, R ? y[t][m] + k * acc[t] : y[t][m], at[t][m]);
+                ad_f4 z = y[m][t];
+                if (R) z += *(const ad_f4 *)&tile[wave][8 * t + yrow][4 * (lane & 7)];
+                ad_out4(j, ob, z, at[m][t]);
             }
         }
     }

@@ -215,23 +215,42 @@ struct PieceView {
     static constexpr int V = F16 ? 8 : 4, NV = kPiece / NT / V + 1, N = NV * V;
     const uint4 *q;
     int first, off, len;  // token of the border, piece's first token behind it, its tokens
+    bool whole;           // nothing to mask: NV - 1 full vectors
     __device__ __forceinline__ PieceView(const void *logits, size_t base, int p, int n) {
         const size_t at = base + (size_t)p * kPiece;
         off = (int)(at % V);
         first = p * kPiece - off;
         len = min(kPiece, n - p * kPiece);
+        whole = off == 0 && len == kPiece;
         q = (const uint4 *)((const char *)logits + (at - off) * (F16 ? 2 : 4));
     }
     __device__ __forceinline__ int token(int x) const { return first + ((int)threadIdx.x + NT * (x / V)) * V + x % V; }
+    // past the piece's end its last vector again
     __device__ __forceinline__ void load(uint4 (&r)[NV]) const {
+        const int last = (len + off - 1) / V;
 #pragma unroll
-        for (int b = 0; b < NV; b++) {
-            const int vec = (int)threadIdx.x + NT * b;
-            if (vec * V < len + off) r[b] = q[vec];
+        for (int b = 0; b < NV - 1; b++) r[b] = q[min((int)threadIdx.x + NT * b, last)];
+        if (off) r[NV - 1] = q[min((int)threadIdx.x + NT * (NV - 1), last)];
+    }
+    // which of a thread's tokens X0 to X1 - 1 are in a range: X1 - 1 in the lowest bit; a NaN is not
+    template <int X0, int X1>
+    static __device__ __forceinline__ uint32_t within(const uint4 (&r)[NV], float lo, float hi) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int x = X0; x < X1; x++) {
+            const float l = raw_value<F16>(r[x / V], x % V);
+            hits = hits + hits + (__builtin_amdgcn_fmed3f(l, lo, hi) == l);
         }
+        return hits;
     }
     // sets what is not the piece's to -inf
     __device__ __forceinline__ void edges(uint4 (&r)[NV]) const {
+        if (off == 0) r[NV - 1] = make_uint4(0,0,0,0);
+        if (whole) {
+            constexpr uint32_t none = F16 ? 0xFC00FC00u : 0xFF800000u;
+            r[NV - 1] = make_uint4(none, none, none, none);
+            return;
+        }
 #pragma unroll
         for (int b = 0; b < NV; b++) {
             const int i = ((int)threadIdx.x + NT * b) * V;
@@ -361,6 +380,12 @@ struct DrawCut {
     __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
 
+struct DrawPair {
+    uint32_t key, idx;
+    uint64_t w;
+};
+constexpr int kDirect = 128;  // tokens resolved each against all others: 2048 pairs a wave at most
+constexpr int kWhole = 1024;  // tokens listed down from the maximum, for a second cut among them
 constexpr int kFew = 8;  // pieces whose histograms and tokens are held at once (n <= 65536)
 // Eight bins a lane, with a gap behind each eight against bank conflicts.
 __device__ __forceinline__ int bin_at(int b) { return b + (b >> 3); }
@@ -387,6 +412,7 @@ struct __align__(16) PickShared {
     union {
         struct {
             uint32_t list_key[kListRoom], list_idx[kListRoom];  // tokens of one bin
+            DrawPair pair[kDirect];
         };
         float tok[kPiece + kPiece / 8 + 16];  // at last the draw's piece
     };
@@ -395,6 +421,7 @@ struct __align__(16) PickShared {
     double before_d;
     uint64_t before_u, wave_total[kPickThreads / 64];
     uint32_t at, ties;
+    DrawCut cut;
 };
 
 // In wave 0: the first of 512 parts (eight a lane) at which `before` and what
@@ -534,8 +561,9 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
         uint64_t want = 0, before = 0;
         bool limited = false;
         DrawCut lim = cut;
-        int listed = -1;  // the bin in the list, with its keys from list_lo to list_hi
+        bool listed = false;  // the list holds all tokens with keys from list_lo to list_hi
         uint32_t list_lo = 0, list_hi = 0;
+        bool above = false;   // list what is above the bin too
         for (;;) {
             const bool by_count = stage == 0;
             if (mode == kNext) {
@@ -613,6 +641,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                     want = counts ? (uint64_t)left : (uint64_t)ceil(ldexp(left, (bin >> 3) + kInBits - kCutBits));
                     before = 0;
                     mode = kNarrow;
+                    above = counts && d.top_p < 1.0f && before_d + cnt <= kWhole;
                 } else {
                     mode = kKeep;
                 }
@@ -638,33 +667,36 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
             // a pass over the bin's tokens with keys in [klo, khi]: from the list,
             // into which a bin of at most kList tokens goes whole, a larger one
             // half a piece at a time
-            const bool held = listed == bin && klo >= list_lo && khi <= list_hi;
+            const bool held = listed && klo >= list_lo && khi <= list_hi;
             __syncthreads();
             if (mode != kKeep)
                 for (int b = tid; b < kBinRoom; b += NT) S.sub_sum[b] = 0, S.sub_cnt[b] = 0;
-            if (tid == 0) S.ntodo = 0, S.list_n = held ? S.list_n : 0;
+            if (tid == 0) S.ntodo = 0, S.list_n = held ? S.list_n : 0, S.before_u = 0;
             __syncthreads();
             int chunks = 1;
+            bool direct = false;
             if (!held) {
+                list_lo = klo;
+                list_hi = above ? lg_key(m) : khi;
                 if (tid < P) {
                     const int b = bin - S.shift[tid];
-                    if (b >= 0 && piece_bin(tid, b)) S.todo[atomicAdd(&S.ntodo, 1)] = tid;
+                    if (above ? lg_key(mine_p.m) >= klo : b >= 0 && piece_bin(tid, b)) S.todo[atomicAdd(&S.ntodo, 1)] = tid;
                 }
+                above = false;
                 __syncthreads();
-                listed = -1;
-                if (cnt <= kList)
-                    listed = bin, list_lo = klo, list_hi = khi;
-                else
+                listed = cnt <= kList;
+                if (!listed)
                     chunks = 2 * S.ntodo;  // kListRoom tokens each at most
             }
             const DrawUnit in_unit(d.c, e - (double)kSteps * (bin >> 3), m);
             for (int ch = 0; ch < chunks; ch++) {
                 if (!held) {
-                    const int t0 = listed >= 0 ? 0 : ch >> 1, t1 = listed >= 0 ? S.ntodo : t0 + 1;
-                    // the masks below hold 16 tokens of a thread: of a piece's 32 and a vector, half a piece is the first
-                    constexpr int kMask = 16;
-                    auto ch_mask = [&](int x0) { return listed >= 0 || (x0 >= kMask) == (ch & 1) ? ~0u : 0u; };
-                    const float llo = lg_unkey(klo), lhi = lg_unkey(khi);
+                    const int t0 = listed ? 0 : ch >> 1, t1 = listed ? S.ntodo : t0 + 1;
+                    // half a piece is each thread's first or last 16 tokens, these with what lies behind the last border
+                    constexpr int PT = kPiece / NT;
+                    static_assert(PT == 32);
+                    const uint32_t half = listed ? ~0u : ch & 1 ? 0xFFFFu : 0xFFFF0000u;
+                    const float llo = lg_unkey(list_lo), lhi = lg_unkey(list_hi);
                     if (ch) {
                         __syncthreads();
                         if (tid == 0) S.list_n = 0;
@@ -679,25 +711,20 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
 #pragma unroll
                         for (int a = 0; a < AT; a++) {
                             if (t + a >= t1) break;
-                            const View view(logits, base, S.todo[t + a], n);
-                            view.edges(raw[a]);
-#pragma unroll
-                            for (int x0 = 0; x0 < View::N; x0 += kMask) {
-                                constexpr int M = kMask;
-                                uint32_t hits = 0;  // tokens in the range, the first one in the highest bit
-#pragma unroll
-                                for (int x = x0; x < x0 + M && x < View::N; x++) {
-                                    const float l = raw_value<F16>(raw[a][x / View::V], x % View::V);
-                                    hits = hits + hits + (__builtin_amdgcn_fmed3f(l, llo, lhi) == l);  // a NaN is not
-                                }
-                                hits &= ch_mask(x0);
+                            const int p = S.todo[t + a];
+                            const View view(logits, base, p, n);
+                            auto list = [&](uint32_t hits, int x0) {
                                 while (hits) {
-                                    const int z = __clz((int)hits), x = x0 + z - (32 - min(M, View::N - x0));
+                                    const int z = __clz((int)hits);
                                     hits &= ~(0x80000000u >> z);
+                                    const uint32_t i = view.token(x0 + z);
+                                    if (i - p * kPiece >= (uint32_t)view.len) continue;  // a neighbour's
                                     const uint32_t at = atomicAdd(&S.list_n, 1u);
-                                    if (at < kListRoom) S.list_idx[at] = view.token(x);
+                                    if (at < kListRoom) S.list_idx[at] = i;
                                 }
-                            }
+                            };
+                            list(View::template within<0, PT>(raw[a], llo, lhi) & half, 0);
+                            if (view.off && (half & 1)) list(View::template within<PT, View::N>(raw[a], llo, lhi), PT - (32 - View::V));
                         }
                     }
                     __syncthreads();
@@ -705,6 +732,40 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                 const uint32_t have = min(S.list_n, (uint32_t)kListRoom);
                 if (!held)  // their keys, all loads at once; below a thread meets its own
                     for (uint32_t x = tid; x < have; x += NT) S.list_key[x] = lg_key(lg_value<F16>(logits, base + S.list_idx[x]));
+                if (mode == kNarrow && listed && have <= kDirect) {
+                    // few tokens: each against all others gives what is ahead of it, and so the cut
+                    uint64_t w = 0;
+                    if (tid < (int)have) {
+                        const uint32_t k = S.list_key[tid], i = S.list_idx[tid];
+                        int down;
+                        if (k >= klo && k <= khi && !(limited && !lim.keeps(k, i))) w = by_count ? 1 : draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down);
+                        S.pair[tid] = DrawPair{k, i, w};
+                        atomicAdd((unsigned long long *)&S.before_u, (unsigned long long)w);
+                    }
+                    if (tid == 0) S.cut = DrawCut{klo, 0xFFFFFFFFu};
+                    __syncthreads();
+#pragma unroll
+                    for (int x0 = 0; x0 < kDirect; x0 += 64) {
+                        if (x0 >= (int)have) break;
+                        const DrawPair own = S.pair[x0 + lane];
+                        uint64_t s = 0;
+                        for (int y = wave; y < (int)have; y += NW) {
+                            const DrawPair o = S.pair[y];
+                            s += o.key > own.key || (o.key == own.key && o.idx < own.idx) ? o.w : 0;
+                        }
+                        atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
+                    }
+                    __syncthreads();
+                    const uint64_t to = min(want > before ? want - before : 1, S.before_u), b = tid < kDirect ? S.sub_sum[tid] : 0;
+                    if (w && b < to && to <= b + w) S.cut = DrawCut{S.list_key[tid], S.list_idx[tid]};
+                    __syncthreads();
+                    cut = S.cut;
+                    cbin = bin;
+                    cnt = S.cnt[bin_at(bin)];
+                    mode = kKeep;
+                    direct = true;
+                    break;
+                }
                 for (uint32_t x = tid; x < have; x += NT) {
                     const uint32_t k = S.list_key[x], i = S.list_idx[x];
                     if (k < klo || k > khi) continue;
@@ -723,6 +784,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                     atomicAdd((unsigned long long *)(keep ? &S.kept[p] : &S.sub_sum[part]), (unsigned long long)w);
                 }
             }
+            if (direct) continue;
             __syncthreads();
             if (mode == kKeep) {
                 mode = kNext;
@@ -879,13 +941,16 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
         const View view(logits, base, piece, n);
         uint4 raw[View::NV];
         view.load(raw);
-        float v[View::N];
-        view.values(raw, v);
         // position j of the view (token view.first + j) at j + 4 (j / 32): 16-byte writes and reads, all banks
 #pragma unroll
         for (int x = 0; x < View::N; x += 4) {
             const int j = (tid + NT * (x / View::V)) * View::V + x % View::V;
-            if (j < kPiece + 8) *(float4 *)&S.tok[j + 4 * (j >> 5)] = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+            float4 l;
+            l.x = raw_value<F16>(raw[x / View::V], x % View::V);
+            l.y = raw_value<F16>(raw[x / View::V], x % View::V + 1);
+            l.z = raw_value<F16>(raw[x / View::V], x % View::V + 2);
+            l.w = raw_value<F16>(raw[x / View::V], x % View::V + 3);
+            if (j < kPiece + view.off) *(float4 *)&S.tok[j + 4 * (j >> 5)] = l;
         }
         __syncthreads();
         constexpr int PT = kPiece / NT;
@@ -900,9 +965,12 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
 #pragma unroll
             for (int y = 0; y < 4; y++) keep |= l[y] > lc || (l[y] == lc && i0 + x + y <= cut.last) ? 1u << (x + y) : 0;
         }
+        // the piece's own only
+        const int skip = tid ? 0 : view.off, end = view.off + view.len - tid * PT;
+        keep = end <= 0 ? 0 : keep >> skip << skip & (end < PT ? (1u << end) - 1 : ~0u);
         // the last thread has the tokens behind the last border too
         if (view.off && tid == NT - 1)
-            for (int x = 0; x < 8; x++) {
+            for (int x = 0; x < end - PT; x++) {
                 const float l = own[PT + 4 + x];
                 more |= l > lc || (l == lc && i0 + PT + x <= cut.last) ? 1u << x : 0;
             }

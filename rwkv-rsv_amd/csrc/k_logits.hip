@@ -199,6 +199,15 @@ __device__ __forceinline__ T wave_scan(T v) {
     v += dpp64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 template <typename T>
 __device__ __forceinline__ T lane_of(T v, int lane) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -242,6 +251,21 @@ struct PieceView {
             hits = hits + hits + (__builtin_amdgcn_fmed3f(l, lo, hi) == l);
         }
         return hits;
+    }
+    // takes a neighbour's tokens out of within<0, N - V> and within<N - V, N>
+    __device__ __forceinline__ void own(uint32_t &hits, uint32_t &more) const {
+        uint32_t mask = 0;
+#pragma unroll
+        for (int b = 0; b < NV; b++) {
+            const int i = ((int)threadIdx.x + NT * b) * V;  // behind the border
+            const int lo = min(max(off - i, 0), V), hi = min(max(len + off - i, 0), V);
+            const uint32_t in = hi > lo ? (1u << (V - lo)) - (1u << (V - hi)) : 0;
+            if (b == NV - 1)
+                more &= in;
+            else
+                mask = mask << V | in;
+        }
+        hits &= mask;
     }
     // sets what is not the piece's to -inf
     __device__ __forceinline__ void edges(uint4 (&r)[NV]) const {
@@ -708,23 +732,36 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
 #pragma unroll
                         for (int a = 0; a < AT; a++)
                             if (t + a < t1) View(logits, base, S.todo[t + a], n).load(raw[a]);
+                        uint32_t hits[AT], more[AT], own = 0;
 #pragma unroll
                         for (int a = 0; a < AT; a++) {
-                            if (t + a >= t1) break;
-                            const int p = S.todo[t + a];
-                            const View view(logits, base, p, n);
-                            auto list = [&](uint32_t hits, int x0) {
-                                while (hits) {
-                                    const int z = __clz((int)hits);
-                                    hits &= ~(0x80000000u >> z);
-                                    const uint32_t i = view.token(x0 + z);
-                                    if (i - p * kPiece >= (uint32_t)view.len) continue;  // a neighbour's
-                                    const uint32_t at = atomicAdd(&S.list_n, 1u);
-                                    if (at < kListRoom) S.list_idx[at] = i;
-                                }
-                            };
-                            list(View::template within<0, PT>(raw[a], llo, lhi) & half, 0);
-                            if (view.off && (half & 1)) list(View::template within<PT, View::N>(raw[a], llo, lhi), PT - (32 - View::V));
+                            hits[a] = more[a] = 0;
+                            if (t + a >= t1) continue;
+                            const View view(logits, base, S.todo[t + a], n);
+                            hits[a] = View::template within<0, PT>(raw[a], llo, lhi) & half;
+                            if (view.off && (half & 1)) more[a] = View::template within<PT, View::N>(raw[a], llo, lhi);
+                            if (!view.whole) view.own(hits[a], more[a]);
+                            own += __popc(hits[a]) + __popc(more[a]);
+                        }
+                        const uint32_t end = wave_scan32(own), all = __builtin_amdgcn_readlane((int)end, 63);
+                        if (all == 0) continue;
+                        uint32_t at = 0;
+                        if (lane == 0) at = atomicAdd(&S.list_n, all);
+                        at = __builtin_amdgcn_readfirstlane((int)at) + end - own;
+#pragma unroll
+                        for (int a = 0; a < AT; a++) {
+                            if (t + a >= t1) continue;
+                            const View view(logits, base, S.todo[t + a], n);
+                            for (uint32_t h = hits[a]; h;) {
+                                const int z = __clz((int)h);
+                                h &= ~(0x80000000u >> z);
+                                if (at < kListRoom) S.list_idx[at++] = view.token(z);
+                            }
+                            for (uint32_t h = more[a]; h;) {
+                                const int z = __clz((int)h);
+                                h &= ~(0x80000000u >> z);
+                                if (at < kListRoom) S.list_idx[at++] = view.token(z + PT - (32 - View::V));
+                            }
                         }
                     }
                     __syncthreads();
@@ -735,12 +772,14 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                 if (mode == kNarrow && listed && have <= kDirect) {
                     // few tokens: each against all others gives what is ahead of it, and so the cut
                     uint64_t w = 0;
-                    if (tid < (int)have) {
+                    if (wave < kDirect / 64) {
                         const uint32_t k = S.list_key[tid], i = S.list_idx[tid];
                         int down;
-                        if (k >= klo && k <= khi && !(limited && !lim.keeps(k, i))) w = by_count ? 1 : draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down);
+                        if (tid < (int)have && k >= klo && k <= khi && !(limited && !lim.keeps(k, i)))
+                            w = by_count ? 1 : draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down);
                         S.pair[tid] = DrawPair{k, i, w};
-                        atomicAdd((unsigned long long *)&S.before_u, (unsigned long long)w);
+                        const uint64_t all = wave_scan(w);
+                        if (lane == 63) atomicAdd((unsigned long long *)&S.before_u, (unsigned long long)all);
                     }
                     if (tid == 0) S.cut = DrawCut{klo, 0xFFFFFFFFu};
                     __syncthreads();
@@ -749,9 +788,12 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                         if (x0 >= (int)have) break;
                         const DrawPair own = S.pair[x0 + lane];
                         uint64_t s = 0;
-                        for (int y = wave; y < (int)have; y += NW) {
-                            const DrawPair o = S.pair[y];
-                            s += o.key > own.key || (o.key == own.key && o.idx < own.idx) ? o.w : 0;
+                        for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
+#pragma unroll
+                            for (int y = 0; y < 8; y++) {
+                                const DrawPair o = S.pair[y0 + 8 * wave + y];  // without weight behind the last
+                                s += o.key > own.key || (o.key == own.key && o.idx < own.idx) ? o.w : 0;
+                            }
                         }
                         atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
                     }

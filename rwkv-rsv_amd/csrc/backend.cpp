@@ -1840,6 +1840,9 @@ static int logits_limits(uint64_t n, uint64_t rows, const char *what) {
         return RSV_FAIL("%s: n=%llu outside 1..%llu", what, (unsigned long long)n, (unsigned long long)kLogitsMaxN);
     if (rows == 0 || rows > kAdapterRows)
         return RSV_FAIL("%s: %llu rows outside 1..%llu", what, (unsigned long long)rows, (unsigned long long)kAdapterRows);
+    if (rows * ((n + 8191) / 8192) > kLogitsMaxPieces)
+        return RSV_FAIL("%s: %llu rows of %llu are more than %llu pieces of 8192", what, (unsigned long long)rows,
+                        (unsigned long long)n, (unsigned long long)kLogitsMaxPieces);
     return 0;
 }
 

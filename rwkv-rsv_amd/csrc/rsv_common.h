@@ -320,7 +320,7 @@ struct AdapterJobs {
 uint64_t adapter_work_words(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t rank, uint64_t rows);
 int launch_adapter(rsv_ctx *ctx, AdapterJobs &J, const rsv_adapter_job *jobs, float *work);
 // Draws and log-probabilities from logits rows (k_logits.hip).
-constexpr uint64_t kLogitsMaxN = (uint64_t)1 << 20;
+constexpr uint64_t kLogitsMaxN = (uint64_t)1 << 20, kLogitsMaxPieces = (uint64_t)1 << 22;  // a block a piece: fewer than 2^32 threads
 uint64_t logits_work_words(uint64_t n, uint64_t rows);
 int launch_draw(rsv_ctx *ctx, const void *logits, int f16, uint32_t *token, uint64_t n, const float *filter,
                 const float *rnd, float *logp, float *work, uint64_t rows);

@@ -42,3 +42,13 @@ def test_null_context(name, nargs):
     assert len(args) == nargs
     assert fn(None, *args) != 0
     assert b"null context" in rsv.hip_lib().rsv_last_error()
+
+
+def test_logits_pieces_limit():
+    """A block takes a piece of 8192: more than 2^22 pieces are refused, that many are not."""
+    import rsv
+    lib = rsv.hip_lib()
+    assert lib.rsv_logits_work(65536, 1 << 19) > 0
+    assert lib.rsv_logits_work(65536, (1 << 19) + 1) == 0
+    assert b"pieces" in lib.rsv_last_error()
+    assert lib.rsv_logits_work(8193, 1 << 20) > 0 and lib.rsv_logits_work(1048576, 1 << 20) == 0

@@ -463,7 +463,7 @@ constexpr int kUpThreads = 256, kUpN = 128;
 // h of row p of a group into hi, lo and back: four lanes a row (c), eights of
 // ranks each.  src: the window row; live: the row is the group's.
 template <int RU>
-__device__ __forceinline__ void ad_stage(const AdapterJobs &J, const AdapterJob &j, int win, int Q, int R, float scale, int p, int c,
+__device__ __forceinline__ void ad_stage(const AdapterJobs &J, const AdapterJob &j, int win, int Q, int R, int p, int c,
                                          uint32_t src, bool live, _Float16 (*hi)[32 * RU + 8], _Float16 (*lo)[32 * RU + 8], float *back) {
     const uint32_t hrow = live ? src * J.rank * 4u + 32 * c : kOff;
     ad_f4 v[RU][2] = {};
@@ -501,7 +501,7 @@ __device__ __forceinline__ void ad_stage(const AdapterJobs &J, const AdapterJob 
         *(ad_h8 *)&hi[p][32 * u + 8 * c] = a;
         *(ad_h8 *)&lo[p][32 * u + 8 * c] = z;
     }
-    if (c == 0) back[p] = scale * __uint_as_float((uint32_t)(127 + ex) << 23);
+    if (c == 0) back[p] = __uint_as_float((uint32_t)(127 + ex) << 23);
 }
 
 // Four neighbouring n of a row of y (elements at `at` of the window), and the outputs.
@@ -534,7 +534,7 @@ template <int RU, bool ONE>  // 32-rank units; one block for all groups of a win
 __global__ __launch_bounds__(kUpThreads, RU <= 2 ? 4 : 2) void k_adapter_up(AdapterJobs J, int slots) {
     constexpr int HS = 32 * RU + 8;
     __shared__ __align__(16) _Float16 hi[kWin][HS], lo[kWin][HS];
-    __shared__ float back[kWin];  // scale times the row's power of two
+    __shared__ float back[kWin];  // the row's power of two
     __shared__ __align__(16) float tile[kUpThreads / 64][16][36];
     const int slot = ONE ? 0 : blockIdx.z / J.njob, step = ONE ? 1 : slots;
     const AdapterJob &j = J.j[ONE ? blockIdx.z : blockIdx.z % J.njob];
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(kUpThreads, RU <= 2 ? 4 : 2) void k_adapter_up(Adap
         if (R) {
             const int p = threadIdx.x >> 2;
             const uint32_t src = __builtin_amdgcn_ds_bpermute(4 * p, grp.row);  // all lanes take part
-            ad_stage<RU>(J, j, win, Q, R, grp.scale, p, threadIdx.x & 3, src, p < grp.cnt, hi, lo, back);
+            ad_stage<RU>(J, j, win, Q, R, p, threadIdx.x & 3, src, p < grp.cnt, hi, lo, back);
             __syncthreads();
             ad_clear_past(b[0], R, g);
             ad_clear_past(b[1], R, g);
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(kUpThreads, RU <= 2 ? 4 : 2) void k_adapter_up(Adap
             if (R) {
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-                for (int t = 0; t < 2; t++) *(ad_f4 *)&tile[wave][i][16 * t + 4 * g] = back[p] * acc[t];
+                for (int t = 0; t < 2; t++) *(ad_f4 *)&tile[wave][i][16 * t + 4 * g] = grp.scale * (back[p] * acc[t]);
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
 #pragma unroll

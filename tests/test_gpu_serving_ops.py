@@ -206,6 +206,20 @@ def test_adapters_in_place_and_non_finite_rows(be, tens, rows):
     assert not np.isfinite(got[2]).any() and np.isnan(got[5, 3]) and np.isfinite(np.delete(got[5], 3)).all()
 
 
+@pytest.mark.parametrize("rows", [6, 100])
+def test_adapters_large_scale_beside_small_weights(be, tens, rows):
+    """scale times h is past fp32's range, their product with b is not: 1e12 * 1e30 * 1e-4."""
+    rng = np.random.default_rng(3)
+    c = Adapters(tens, rng, rows, 2, 8, [(64, 136)], ranks=[1, 1])
+    c.scale[:] = 1e12
+    a, b, x, _ = c.host[0]
+    a[:], x[:] = 1.0, np.float32(1e30 / 64) * rng.uniform(0.5, 1.0, x.shape).astype(np.float32)
+    b[:] = np.float16(1e-4)
+    c.upload()
+    c.call(be)
+    c.check(be)
+
+
 def test_adapters_far_offsets(be, tens):
     """An adapter whose matrices lie past 2^31 elements of the pool."""
     import rsv

@@ -536,6 +536,18 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
     __syncthreads();
     const DrawUnit unit(d.c, e, m);
     const float low = draw_low(m, d);
+    const double uu = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+    // ln of the probability of l among kept weights of this sum in the row's
+    // unit: total 2^(E - bits), the maximum lies `below` octaves under E
+    auto log_p = [&](float l, double total, int bits) {
+        double below = 1.0;
+        if (!unit.sharp) {
+            double r;
+            below = -(double)unit.steps(m, r);
+            below = (below - r) / kSteps;
+        }
+        return (float)((l == m ? 0.0 : ((double)l - (double)m) / d.T) - (log(ldexp(total, -bits)) + below * 0.69314718055994530942));
+    };
     const double inv_c = d.T * (0.69314718055994530942 / kSteps);
     DrawCut cut{0, 0xFFFFFFFFu};
     int cbin = kBins;  // the cut's bin; kBins: no cut
@@ -579,15 +591,17 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
         // passes over the bin's tokens (kNarrow), finds the last of that key's
         // tokens if some have to go (kTies), and sums up what the pieces keep
         // (kKeep).
-        enum { kNext, kNarrow, kTies, kKeep };
+        enum { kNext, kNarrow, kTies, kKeep, kAll };
         int mode = kNext, stage = -1, bin = 0, sh = 0;
         uint32_t klo = 0, khi = 0, top_key = 0, cnt = 0, ties = 0, count = 0, ilo = 0, ihi = 0, step = 0;
         uint64_t want = 0, before = 0;
+        double row_goal = 0.0;  // kAll: top-p's of the whole row
         bool limited = false;
         DrawCut lim = cut;
         bool listed = false;  // the list holds all tokens with keys from list_lo to list_hi
         uint32_t list_lo = 0, list_hi = 0;
         bool above = false;   // list what is above the bin too
+        bool fresh = true;    // before the row's first cut
         for (;;) {
             const bool by_count = stage == 0;
             if (mode == kNext) {
@@ -669,7 +683,19 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                 } else {
                     mode = kKeep;
                 }
-                if (mode == kNarrow) continue;
+                if (fresh) {  // few tokens down to the bin: they settle the row
+                    fresh = false;
+                    uint32_t c = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) c += 8 * lane + j <= bin ? S.cnt[9 * lane + j] : 0;
+                    if (__builtin_amdgcn_readlane((int)wave_scan32(c), 63) <= kDirect) {
+                        if (mode == kKeep) klo = cut.key, khi = max(top_key, klo);
+                        mode = kAll;
+                        above = true;
+                        row_goal = goal;
+                    }
+                }
+                if (mode != kKeep) continue;
             }
             if (mode == kKeep) {  // whole bins; the cut's own token by token
                 for (int p = wave; p < P; p += NW) {
@@ -685,7 +711,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
             } else if (mode == kNarrow) {
                 sh = 0;
                 while ((khi - klo) >> sh >= kBins) sh++;
-            } else {
+            } else if (mode == kTies) {
                 step = (ihi - ilo) / kBins + 1;
             }
             // a pass over the bin's tokens with keys in [klo, khi]: from the list,
@@ -769,6 +795,84 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                 const uint32_t have = min(S.list_n, (uint32_t)kListRoom);
                 if (!held)  // their keys, all loads at once; below a thread meets its own
                     for (uint32_t x = tid; x < have; x += NT) S.list_key[x] = lg_key(lg_value<F16>(logits, base + S.list_idx[x]));
+                if (mode == kAll) {
+                    // each token against all others, in the row's order and by index: both cuts and the draw
+                    uint64_t w = 0;
+                    uint32_t k = 0, i = 0;
+                    if (tid < kDirect) {
+                        if (tid < (int)have) {
+                            int down;
+                            k = S.list_key[tid], i = S.list_idx[tid];
+                            w = draw_weight(unit, lg_unkey(k), kPlainBits, S.tab, down);
+                        }
+                        S.pair[tid] = DrawPair{k, i, w};
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int x0 = 0; x0 < kDirect; x0 += 64) {
+                        if (x0 >= (int)have) break;
+                        const DrawPair own = S.pair[x0 + lane];
+                        uint64_t s = 0;
+                        uint32_t c = 0;
+                        for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
+#pragma unroll
+                            for (int y = 0; y < 8; y++) {
+                                const DrawPair o = S.pair[y0 + 8 * wave + y];  // key 0 behind the last
+                                const bool ahead = o.key > own.key || (o.key == own.key && o.idx < own.idx && o.key);
+                                s += ahead ? o.w : 0;
+                                c += ahead;
+                            }
+                        }
+                        atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
+                        atomicAdd(&S.sub_cnt[x0 + lane], c);
+                    }
+                    __syncthreads();
+                    uint64_t ahead = 0;
+                    bool in = tid < (int)have;
+                    bool top = false;  // the first of all
+                    if (tid < kDirect) {
+                        const uint32_t c = S.sub_cnt[tid];
+                        ahead = S.sub_sum[tid];
+                        S.sub_sum[tid] = 0;
+                        top = c == 0;
+                        in = in && (!d.top_k || c < d.top_k);
+                        const uint64_t all = wave_scan(in ? w : 0);
+                        if (lane == 63) S.wave_total[wave] = all;
+                    }
+                    __syncthreads();
+                    if (tid < kDirect) {
+                        const uint64_t all = S.wave_total[0] + S.wave_total[1];
+                        const double lim_p = stage == 1 ? ldexp(row_goal, kPlainBits - kCutBits) : (double)d.top_p * (double)all;
+                        in = in && (d.top_p >= 1.0f || top || (double)ahead < lim_p);
+                        if (!in) w = 0;
+                        S.pair[tid].w = w;
+                        const uint64_t kept = wave_scan(w);
+                        if (lane == 63) S.wave_total[2 + wave] = kept;
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int x0 = 0; x0 < kDirect; x0 += 64) {
+                        if (x0 >= (int)have) break;
+                        const uint32_t own = S.pair[x0 + lane].idx;
+                        uint64_t s = 0;
+                        for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
+#pragma unroll
+                            for (int y = 0; y < 8; y++) {
+                                const DrawPair o = S.pair[y0 + 8 * wave + y];
+                                s += o.idx < own ? o.w : 0;
+                            }
+                        }
+                        atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
+                    }
+                    __syncthreads();
+                    const uint64_t total = S.wave_total[2] + S.wave_total[3], run = tid < kDirect ? S.sub_sum[tid] : 0;
+                    const uint64_t goal = min((uint64_t)(uu * (double)total), total - 1);
+                    if (w && run <= goal && goal < run + w) {
+                        token[row] = i;
+                        if (logp) logp[row] = log_p(lg_unkey(k), (double)total, kPlainBits);
+                    }
+                    return;
+                }
                 if (mode == kNarrow && listed && have <= kDirect) {
                     // few tokens: each against all others gives what is ahead of it, and so the cut
                     uint64_t w = 0;
@@ -902,7 +1006,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
 #pragma unroll
         for (int x = 0; x < 8; x++) total += (double)S.kept[p0 + x] * S.scale[p0 + x];
     }
-    const double target = (double)(u > 0.0f ? fminf(u, 1.0f) : 0.0f) * total;
+    const double target = uu * total;
     double run = 0.0, gone = 0.0;
     int piece = -1;
     for (int p0 = 0; p0 < P; p0 += 8) {
@@ -912,14 +1016,6 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
             if (s > 0.0 && run <= target) piece = p0 + x, gone = run;
             run += s;
         }
-    }
-    // ln of the kept sum beside the maximum: total 2^(E - bits), the maximum
-    // lies `below` octaves under E
-    double below = 1.0;
-    if (!unit.sharp) {
-        double r;
-        below = -(double)unit.steps(m, r);
-        below = (below - r) / kSteps;
     }
     const DrawUnit pu(d.c, S.piece[piece].e, S.piece[piece].m);
     const float plow = draw_low(S.piece[piece].m, d);
@@ -945,7 +1041,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
         if (goal < b || goal >= b + mine) return;
         float l;
         token[row] = walk(goal - b, l);
-        if (logp) logp[row] = (float)((l == m ? 0.0 : ((double)l - (double)m) / d.T) - (log(ldexp(total, -bits)) + below * 0.69314718055994530942));
+        if (logp) logp[row] = log_p(l, total, bits);
     };
     if (grouped) {
         constexpr int V = 4;

@@ -404,11 +404,7 @@ struct DrawCut {
     __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
 
-struct DrawPair {
-    uint32_t key, idx;
-    uint64_t w;
-};
-constexpr int kDirect = 128;  // tokens resolved each against all others: 2048 pairs a wave at most
+constexpr int kSorted = kPickThreads;  // tokens put in order each against all others: 4096 comparisons a wave at most
 constexpr int kWhole = 1024;  // tokens listed down from the maximum, for a second cut among them
 constexpr int kFew = 8;  // pieces whose histograms and tokens are held at once (n <= 65536)
 // Eight bins a lane, with a gap behind each eight against bank conflicts.
@@ -436,7 +432,8 @@ struct __align__(16) PickShared {
     union {
         struct {
             uint32_t list_key[kListRoom], list_idx[kListRoom];  // tokens of one bin
-            DrawPair pair[kDirect];
+            uint64_t order[kSorted], weight[kSorted];
+            uint32_t entry[kSorted], by_idx[kSorted];
         };
         float tok[kPiece + kPiece / 8 + 16];  // at last the draw's piece
     };
@@ -598,6 +595,41 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
         double row_goal = 0.0;  // kAll: top-p's of the whole row
         bool limited = false;
         DrawCut lim = cut;
+        // a thread's place among the list's tokens that are in, and (upper half) by index
+        auto sort = [&](bool in, uint32_t key, uint32_t idx, uint32_t have) {
+            S.order[tid] = in ? (uint64_t)key << 32 | (uint32_t)~idx : 0;
+            __syncthreads();
+#pragma unroll
+            for (int x0 = 0; x0 < kSorted; x0 += 64) {
+                if (x0 >= (int)have) break;
+                const uint64_t own = S.order[x0 + lane];
+                uint32_t c = 0, by_idx = 0;
+                for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
+#pragma unroll
+                    for (int y = 0; y < 8; y++) {
+                        const uint64_t o = S.order[y0 + 8 * wave + y];
+                        c += o > own;
+                        by_idx += (uint32_t)o > (uint32_t)own;
+                    }
+                }
+                atomicAdd(&S.sub_cnt[x0 + lane], c | by_idx << 16);
+            }
+            __syncthreads();
+            return S.sub_cnt[tid];
+        };
+        auto block_scan = [&](uint64_t v, uint64_t &all) {
+            const uint64_t pre = wave_scan(v);
+            if (lane == 63) S.wave_total[wave] = pre;
+            __syncthreads();
+            uint64_t b = pre;
+            all = 0;
+#pragma unroll
+            for (int y = 0; y < NW; y++) {
+                if (y < wave) b += S.wave_total[y];
+                all += S.wave_total[y];
+            }
+            return b;
+        };
         bool listed = false;  // the list holds all tokens with keys from list_lo to list_hi
         uint32_t list_lo = 0, list_hi = 0;
         bool above = false;   // list what is above the bin too
@@ -688,7 +720,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                     uint32_t c = 0;
 #pragma unroll
                     for (int j = 0; j < 8; j++) c += 8 * lane + j <= bin ? S.cnt[9 * lane + j] : 0;
-                    if (__builtin_amdgcn_readlane((int)wave_scan32(c), 63) <= kDirect) {
+                    if (__builtin_amdgcn_readlane((int)wave_scan32(c), 63) <= kSorted) {
                         if (mode == kKeep) klo = cut.key, khi = max(top_key, klo);
                         mode = kAll;
                         above = true;
@@ -797,113 +829,48 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
                     for (uint32_t x = tid; x < have; x += NT) S.list_key[x] = lg_key(lg_value<F16>(logits, base + S.list_idx[x]));
                 if (mode == kAll) {
                     // each token against all others, in the row's order and by index: both cuts and the draw
-                    uint64_t w = 0;
-                    uint32_t k = 0, i = 0;
-                    if (tid < kDirect) {
-                        if (tid < (int)have) {
-                            int down;
-                            k = S.list_key[tid], i = S.list_idx[tid];
-                            w = draw_weight(unit, lg_unkey(k), kPlainBits, S.tab, down);
-                        }
-                        S.pair[tid] = DrawPair{k, i, w};
+                    const bool in = tid < (int)have;
+                    const uint32_t k = in ? S.list_key[tid] : 0, i = in ? S.list_idx[tid] : 0;
+                    int down;
+                    const uint64_t w = in ? draw_weight(unit, lg_unkey(k), kPlainBits, S.tab, down) : 0;
+                    const uint32_t at = sort(in, k, i, have);
+                    if (in) {
+                        S.weight[at & 0xFFFF] = w;
+                        S.entry[at & 0xFFFF] = at >> 16;
+                        S.by_idx[at >> 16] = tid;
                     }
                     __syncthreads();
-#pragma unroll
-                    for (int x0 = 0; x0 < kDirect; x0 += 64) {
-                        if (x0 >= (int)have) break;
-                        const DrawPair own = S.pair[x0 + lane];
-                        uint64_t s = 0;
-                        uint32_t c = 0;
-                        for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
-#pragma unroll
-                            for (int y = 0; y < 8; y++) {
-                                const DrawPair o = S.pair[y0 + 8 * wave + y];  // key 0 behind the last
-                                const bool ahead = o.key > own.key || (o.key == own.key && o.idx < own.idx && o.key);
-                                s += ahead ? o.w : 0;
-                                c += ahead;
-                            }
-                        }
-                        atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
-                        atomicAdd(&S.sub_cnt[x0 + lane], c);
-                    }
+                    // a thread has a place in the row's order ...
+                    uint64_t all, total;
+                    const uint64_t mine = in && (!d.top_k || tid < (int)d.top_k) ? S.weight[tid] : 0;
+                    const uint64_t ahead = block_scan(mine, all) - mine;
+                    const double lim_p = stage == 1 ? ldexp(row_goal, kPlainBits - kCutBits) : (double)d.top_p * (double)all;
+                    if (in) S.order[S.entry[tid]] = d.top_p >= 1.0f || tid == 0 || (double)ahead < lim_p ? mine : 0;
                     __syncthreads();
-                    uint64_t ahead = 0;
-                    bool in = tid < (int)have;
-                    bool top = false;  // the first of all
-                    if (tid < kDirect) {
-                        const uint32_t c = S.sub_cnt[tid];
-                        ahead = S.sub_sum[tid];
-                        S.sub_sum[tid] = 0;
-                        top = c == 0;
-                        in = in && (!d.top_k || c < d.top_k);
-                        const uint64_t all = wave_scan(in ? w : 0);
-                        if (lane == 63) S.wave_total[wave] = all;
-                    }
-                    __syncthreads();
-                    if (tid < kDirect) {
-                        const uint64_t all = S.wave_total[0] + S.wave_total[1];
-                        const double lim_p = stage == 1 ? ldexp(row_goal, kPlainBits - kCutBits) : (double)d.top_p * (double)all;
-                        in = in && (d.top_p >= 1.0f || top || (double)ahead < lim_p);
-                        if (!in) w = 0;
-                        S.pair[tid].w = w;
-                        const uint64_t kept = wave_scan(w);
-                        if (lane == 63) S.wave_total[2 + wave] = kept;
-                    }
-                    __syncthreads();
-#pragma unroll
-                    for (int x0 = 0; x0 < kDirect; x0 += 64) {
-                        if (x0 >= (int)have) break;
-                        const uint32_t own = S.pair[x0 + lane].idx;
-                        uint64_t s = 0;
-                        for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
-#pragma unroll
-                            for (int y = 0; y < 8; y++) {
-                                const DrawPair o = S.pair[y0 + 8 * wave + y];
-                                s += o.idx < own ? o.w : 0;
-                            }
-                        }
-                        atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
-                    }
-                    __syncthreads();
-                    const uint64_t total = S.wave_total[2] + S.wave_total[3], run = tid < kDirect ? S.sub_sum[tid] : 0;
+                    // ... and now one by index
+                    const uint64_t kept = in ? S.order[tid] : 0, run = block_scan(kept, total);
                     const uint64_t goal = min((uint64_t)(uu * (double)total), total - 1);
-                    if (w && run <= goal && goal < run + w) {
-                        token[row] = i;
-                        if (logp) logp[row] = log_p(lg_unkey(k), (double)total, kPlainBits);
+                    if (kept && run - kept <= goal && goal < run) {
+                        const uint32_t x = S.by_idx[tid];
+                        token[row] = S.list_idx[x];
+                        if (logp) logp[row] = log_p(lg_unkey(S.list_key[x]), (double)total, kPlainBits);
                     }
                     return;
                 }
-                if (mode == kNarrow && listed && have <= kDirect) {
-                    // few tokens: each against all others gives what is ahead of it, and so the cut
-                    uint64_t w = 0;
-                    if (wave < kDirect / 64) {
-                        const uint32_t k = S.list_key[tid], i = S.list_idx[tid];
-                        int down;
-                        if (tid < (int)have && k >= klo && k <= khi && !(limited && !lim.keeps(k, i)))
-                            w = by_count ? 1 : draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down);
-                        S.pair[tid] = DrawPair{k, i, w};
-                        const uint64_t all = wave_scan(w);
-                        if (lane == 63) atomicAdd((unsigned long long *)&S.before_u, (unsigned long long)all);
-                    }
+                if (mode == kNarrow && listed && have <= kSorted) {  // the cut without more passes
+                    const uint32_t k = S.list_key[tid], i = S.list_idx[tid];
+                    const bool in = tid < (int)have && k >= klo && k <= khi && !(limited && !lim.keeps(k, i));
+                    int down;
+                    const uint64_t w = !in ? 0 : by_count ? 1 : draw_weight(in_unit, lg_unkey(k), kInBits, S.tab, down);
+                    S.weight[tid] = 0;
                     if (tid == 0) S.cut = DrawCut{klo, 0xFFFFFFFFu};
+                    const uint32_t at = sort(in, k, i, have) & 0xFFFF;
+                    if (in) S.weight[at] = w, S.entry[at] = tid;
                     __syncthreads();
-#pragma unroll
-                    for (int x0 = 0; x0 < kDirect; x0 += 64) {
-                        if (x0 >= (int)have) break;
-                        const DrawPair own = S.pair[x0 + lane];
-                        uint64_t s = 0;
-                        for (int y0 = 0; y0 < (int)have; y0 += 8 * NW) {
-#pragma unroll
-                            for (int y = 0; y < 8; y++) {
-                                const DrawPair o = S.pair[y0 + 8 * wave + y];  // without weight behind the last
-                                s += o.key > own.key || (o.key == own.key && o.idx < own.idx) ? o.w : 0;
-                            }
-                        }
-                        atomicAdd((unsigned long long *)&S.sub_sum[x0 + lane], (unsigned long long)s);
-                    }
-                    __syncthreads();
-                    const uint64_t to = min(want > before ? want - before : 1, S.before_u), b = tid < kDirect ? S.sub_sum[tid] : 0;
-                    if (w && b < to && to <= b + w) S.cut = DrawCut{S.list_key[tid], S.list_idx[tid]};
+                    uint64_t all;
+                    const uint64_t mine = S.weight[tid], run = block_scan(mine, all);
+                    const uint64_t to = min(want > before ? want - before : 1, all);
+                    if (mine && run - mine < to && to <= run) S.cut = DrawCut{S.list_key[S.entry[tid]], S.list_idx[S.entry[tid]]};
                     __syncthreads();
                     cut = S.cut;
                     cbin = bin;

@@ -542,13 +542,13 @@ uint64_t rsv_adapter_work(const rsv_adapter_job *jobs, uint64_t njobs, uint64_t 
  * logp[b] (F32 [batch], or 0xFFFFFFFF for none) is the logarithm of the
  * probability that the token had among the kept ones (0 where greedy).
  * Weights are held as integers (their last bit at most 2^-47 of the largest of
- * each 8192 tokens, 2^-36 in rows where a setting cuts) and added up in an
- * order that n alone sets, so a row's draw depends
- * on nothing but its logits, settings and u: not on its place in the batch,
- * nor on the batch.
- * 1 <= n <= 1048576, 1 <= batch <= 1048576, and batch rows of ceil(n / 8192)
- * pieces make 4194304 pieces at most.  work: an F32 tensor of at least rsv_logits_work floats,
- * the caller's, as for rsv_adapter_multi. */
+ * each 8192 tokens, 2^-36 in rows where a setting cuts; less than half of it is
+ * no weight) and added up in an order that n alone sets, so a row's draw
+ * depends on nothing but its logits, settings and u: not on its place in the
+ * batch, nor on the batch.
+ * 1 <= n <= 1048576, 1 <= batch <= 1048576, and the batch's rows, each of
+ * ceil(n / 8192) pieces, make 4194304 pieces at most.  work: an F32 tensor of
+ * at least rsv_logits_work floats, the caller's, as for rsv_adapter_multi. */
 int rsv_sample_rand_batch(rsv_ctx *ctx, uint32_t logits, uint32_t token, uint64_t n, uint32_t filter,
                           uint32_t rand, uint32_t logp, uint32_t work, uint64_t batch);
 /* filter[row] = the four settings, stream-ordered (as rsv_store_sampler). */

@@ -51,10 +51,24 @@ __device__ __forceinline__ void lg_unpack(uint4 q, float (&v)[F16 ? 8 : 4]) {
 // Two launches.  k_draw_scan: a block per (row, piece of 8192 tokens) leaves
 // the piece's maximum, its sum of weights and, where the row's settings cut
 // anything, its histogram over eighths of an octave of weight.  k_draw_pick: a
-// block per row finds the cut from the histograms, resolves it inside the one
-// bin that holds it, takes the draw's piece from the pieces' kept sums and the
-// token from that piece alone.  So the row is read once, and then what lies in
-// one bin and one piece.
+// block per row finds the cut from the histograms and resolves it inside the
+// one bin that holds it.  So the row is read once, and then the pieces that
+// have tokens in that bin:
+// - at most 256 tokens from the maximum down to the bin (peaked rows, small
+//   top-k): listed together, they settle both cuts and the draw (kAll);
+// - otherwise the bin's tokens are listed (in LDS, 4096 at a time), the cut is
+//   narrowed to one key, the draw's piece follows from the pieces' kept sums and
+//   the token from that piece alone.
+//
+// Bounds.  Many rows without cuts stream: 256 rows of 65536 fp32 logits take 25
+// us in the first launch (2.7 TB/s; the rest is 64-bit float work) and 6.5 in
+// the second.  Rows with cuts are bound by the second launch's chain of reads,
+// barriers and LDS round trips on one CU: of one peaked row's 13 us, 3 are the
+// settings, the pieces and the table, 3 the bin, 6 the listing, 2 the rest; 64
+// mixed rows take 8.4 + 22.  A piece's own list of its largest tokens, made by
+// the first launch, saved 5 us of listing and cost 1.6 there and 1 to 5 in rows
+// that it did not settle.  256 threads: what all waves do alike costs a SIMD's
+// issue slots once a wave, and 16 waves a block took four times as long for it.
 //
 // A token's weight is 2^x, x = l log2(e) / T, held as an integer with `bits`
 // bits below E, a whole octave above the piece's largest x.  With c = 1024
@@ -64,7 +78,9 @@ __device__ __forceinline__ void lg_unpack(uint4 q, float (&v)[F16 ? 8 : 4]) {
 // a Taylor polynomial of degree 3 in an argument below 3.4e-4 (6e-16 off).
 // Adding 2^52 to the scaled weight leaves the integer in the low bits.  Eight
 // 64-bit float operations a token; exp() takes about four times as many.
-// Integers add up the same in any order; pieces are put together in 64-bit
+// Weights that round to nothing have no share: below 2^-49 of the piece's
+// largest, 2^-38 in rows with cuts (whose bins leave a weight 37 bits beside a
+// count).  Integers add up the same in any order; pieces are put together in 64-bit
 // floats in the pieces' order, which depends on n alone.  Bins follow q, so
 // they mean the same in every piece.
 //
@@ -404,7 +420,7 @@ struct DrawCut {
     __device__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
 
-constexpr int kSorted = kPickThreads;  // tokens put in order each against all others: 4096 comparisons a wave at most
+constexpr int kSorted = kPickThreads;  // tokens put in order each against all others: 256 comparisons a lane at most
 constexpr int kWhole = 1024;  // tokens listed down from the maximum, for a second cut among them
 constexpr int kFew = 8;  // pieces whose histograms and tokens are held at once (n <= 65536)
 // Eight bins a lane, with a gap behind each eight against bank conflicts.
@@ -1145,7 +1161,9 @@ __device__ __forceinline__ void lp_write(const LpPart &a, float lt, float *logp,
 }
 
 // A block per (row, piece of 16-byte vectors); with one piece a row, the
-// result itself.
+// result itself.  Bound by the read: 2048 rows of 65536 fp32 logits take 96 us
+// (5.6 TB/s, above the 5.1 of a copy).  Few rows are two short launches, 4.0 +
+// 2.6 us for 8 rows; one exp2 a token, the maximum carried per thread.
 template <bool F16>
 __global__ __launch_bounds__(kLpThreads) void k_logprob(const void *__restrict__ logits, int n, int P,
                                                         const uint32_t *__restrict__ token, float *__restrict__ logp,

@@ -360,7 +360,8 @@ def check_draw(be, tens, l, filters, u, kind="f32"):
     for r in range(len(l)):
         want, lp = draw64(l[r], *filters[r], u[r])
         assert tok[r] == want, (r, filters[r], u[r], tok[r], want, l[r][tok[r]] if tok[r] < l.shape[1] else None, l[r][want])
-        # fp64 inside, one rounding to fp32; the integers' last place moves the sum by 2^-62 n at most
+        # fp64 inside, one rounding to fp32; the weights are off by half of 2^-36 of the largest each, either way: root
+        # of 65536 times 0.29 times 2^-36 is 1e-9 of a sum that is not less than the largest
         assert logp[r] == lp or abs(logp[r] - lp) <= 2 * U * abs(lp) + 1e-9, (r, logp[r], lp)
 
 
@@ -397,6 +398,24 @@ def test_draw_nucleus_from_flat_to_peaked(be, tens, spread, top_p):
          (1.0, 30000, top_p, 1e-6)]
     check_draw(be, tens, l, f, rng.random(6))
     check_draw(be, tens, l, f, rng.random(6), "f16")
+
+
+@pytest.mark.parametrize("count", [1, 2, 63, 65, 128, 255, 256, 257, 600, 1024, 1025, 5000])
+@pytest.mark.parametrize("n", [20001, 70001])
+def test_draw_among_few_tokens(be, tens, count, n):
+    """All weight on `count` tokens anywhere in a row, half of them in groups of equal logits; rows that do not start
+    at a 16-byte border."""
+    rng = np.random.default_rng(count * 7 + n)
+    f = [(1.0, 0, 0.9, 0.0), (0.7, count // 2 + 1, 0.8, 0.0), (1.0, count, 1.0, 0.0), (1.0, 0, 0.95, 0.2),
+         (1.0, count + 3, 0.999, 0.0), (2.0, 0, 1.0, 0.5), (1.0, max(1, count // 3), 0.6, 0.3)]
+    l = rng.standard_normal((len(f), n)) - 40.0
+    for r in range(len(f)):
+        at = rng.permutation(n)[:count]
+        v = rng.standard_normal(count) * 0.4
+        v[::2] = np.round(v[::2] * 4) / 4
+        l[r, at] = v
+    check_draw(be, tens, l, f, rng.random(len(f)))
+    check_draw(be, tens, l, f, rng.random(len(f)), "f16")
 
 
 def test_draw_every_token_by_its_share(be, tens):

@@ -231,9 +231,10 @@ __device__ __forceinline__ T lane_of(T v, int lane) {
     return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
 }
 
-// A piece's tokens over NT threads: thread t has the 16-byte vectors t, t + NT,
-// ... from the border at or before the piece's first token on, and one more
-// where the row does not start at a border; tokens that are not the piece's
+// A piece's tokens over NT threads: a wave has a contiguous part, lane l the
+// 16-byte vectors l, l + 64, ... of it, from the border at or before the piece's
+// first token on, and thread t one more behind them where the row does not start
+// at a border; tokens that are not the piece's
 // are -inf.  Vectors stay inside the tensor's memory, whose end is padded.
 template <bool F16, int NT>
 struct PieceView {
@@ -249,13 +250,17 @@ struct PieceView {
         whole = off == 0 && len == kPiece;
         q = (const uint4 *)((const char *)logits + (at - off) * (F16 ? 2 : 4));
     }
-    __device__ __forceinline__ int token(int x) const { return first + ((int)threadIdx.x + NT * (x / V)) * V + x % V; }
+    static __device__ __forceinline__ int vec(int b) {
+        const int t = threadIdx.x;
+        return b == NV - 1 ? NT * (NV - 1) + t : (t >> 6) * (64 * (NV - 1)) + 64 * b + (t & 63);
+    }
+    __device__ __forceinline__ int token(int x) const { return first + vec(x / V) * V + x % V; }
     // past the piece's end its last vector again
     __device__ __forceinline__ void load(uint4 (&r)[NV]) const {
         const int last = (len + off - 1) / V;
 #pragma unroll
-        for (int b = 0; b < NV - 1; b++) r[b] = q[min((int)threadIdx.x + NT * b, last)];
-        if (off) r[NV - 1] = q[min((int)threadIdx.x + NT * (NV - 1), last)];
+        for (int b = 0; b < NV - 1; b++) r[b] = q[min(vec(b), last)];
+        if (off) r[NV - 1] = q[min(vec(NV - 1), last)];
     }
     // which of a thread's tokens X0 to X1 - 1 are in a range: X1 - 1 in the lowest bit; a NaN is not
     template <int X0, int X1>
@@ -273,7 +278,7 @@ struct PieceView {
         uint32_t mask = 0;
 #pragma unroll
         for (int b = 0; b < NV; b++) {
-            const int i = ((int)threadIdx.x + NT * b) * V;  // behind the border
+            const int i = vec(b) * V;  // behind the border
             const int lo = min(max(off - i, 0), V), hi = min(max(len + off - i, 0), V);
             const uint32_t in = hi > lo ? (1u << (V - lo)) - (1u << (V - hi)) : 0;
             if (b == NV - 1)
@@ -293,7 +298,7 @@ struct PieceView {
         }
 #pragma unroll
         for (int b = 0; b < NV; b++) {
-            const int i = ((int)threadIdx.x + NT * b) * V;
+            const int i = vec(b) * V;
             if (i >= off && i + V <= len + off) continue;
             uint32_t w[4] = {r[b].x, r[b].y, r[b].z, r[b].w};
 #pragma unroll
@@ -339,7 +344,6 @@ __global__ __launch_bounds__(kScanThreads) void k_draw_scan(const void *__restri
     if (!d.greedy) draw_table<NT>(tab);
     if (d.cuts)
         for (int b = tid; b < kBins; b += NT) hist[b] = 0;
-    if (tid < kGroups) group[tid] = 0;
     float v[View::N];
     view.values(raw, v);
     float m = v[0];
@@ -389,19 +393,16 @@ __global__ __launch_bounds__(kScanThreads) void k_draw_scan(const void *__restri
         for (int b = tid; b < kBins; b += NT) W.hist[at + b] = hist[b];
         if (tid == 0) out->m = m, out->e = e;
     } else {
-        // a wave's vectors lie in one group, if the row starts at a border
+        // a wave's part is a group, if the row starts at a border
+        static_assert(kPiece / NW == kGroup);
+        uint64_t s = 0;
 #pragma unroll
-        for (int x0 = 0; x0 < View::N; x0 += View::V) {
-            uint64_t s = 0;
-#pragma unroll
-            for (int x = x0; x < x0 + View::V; x++) {
-                int down;
-                if (v[x] >= low) s += draw_weight(unit, v[x], kPlainBits, tab, down);
-            }
-            s = wave_scan(s);
-            const int g = (wave * 64 + NT * (x0 / View::V)) * View::V / kGroup;
-            if (lane == 63 && s) atomicAdd((unsigned long long *)&group[min(g, kGroups - 1)], (unsigned long long)s);
+        for (int x = 0; x < View::N; x++) {
+            int down;
+            if (v[x] >= low) s += draw_weight(unit, v[x], kPlainBits, tab, down);
         }
+        s = wave_scan(s);
+        if (lane == 63) group[wave] = s;
         __syncthreads();
         if (tid < kGroups) out->group[tid] = group[tid];
         if (tid == 0) {
@@ -1065,7 +1066,7 @@ __global__ __launch_bounds__(kPickThreads) void k_draw_pick(const void *__restri
         // position j of the view (token view.first + j) at j + 4 (j / 32): 16-byte writes and reads, all banks
 #pragma unroll
         for (int x = 0; x < View::N; x += 4) {
-            const int j = (tid + NT * (x / View::V)) * View::V + x % View::V;
+            const int j = View::vec(x / View::V) * View::V + x % View::V;
             float4 l;
             l.x = raw_value<F16>(raw[x / View::V], x % View::V);
             l.y = raw_value<F16>(raw[x / View::V], x % View::V + 1);

@@ -396,10 +396,18 @@ __global__ __launch_bounds__(kScanThreads) void k_draw_scan(const void *__restri
         // a wave's part is a group, if the row starts at a border
         static_assert(kPiece / NW == kGroup);
         uint64_t s = 0;
+        if (unit.sharp) {
 #pragma unroll
-        for (int x = 0; x < View::N; x++) {
-            int down;
-            if (v[x] >= low) s += draw_weight(unit, v[x], kPlainBits, tab, down);
+            for (int x = 0; x < View::N; x++) s += v[x] == m ? 1ull << (kPlainBits - 1) : 0;
+        } else {  // every lane weighs, what lies below `low` for nothing
+#pragma unroll
+            for (int x = 0; x < View::N; x++) {
+                if (x >= View::N - View::V && view.off == 0) continue;  // nothing there
+                double r;
+                const int k = unit.steps(v[x], r);
+                const uint64_t w = draw_value(k, r, kPlainBits, tab);
+                s += v[x] >= low ? w : 0;
+            }
         }
         s = wave_scan(s);
         if (lane == 63) group[wave] = s;

@@ -381,12 +381,20 @@ __global__ __launch_bounds__(kScanThreads) void k_draw_scan(const void *__restri
         low = fmaxf(low, f - fabsf(f) * 2.4e-7f);  // NaN beside an infinite m: low stays
     }
     if (d.cuts) {
+        auto add = [&](int down, uint64_t w) { atomicAdd((unsigned long long *)&hist[down >> kBinShift], (unsigned long long)(w | 1ull << 50)); };
+        if (unit.sharp) {
 #pragma unroll
-        for (int x = 0; x < View::N; x++) {
-            if (!(v[x] >= low)) continue;
-            int down;
-            const uint64_t w = draw_weight(unit, v[x], kCutBits, tab, down);
-            atomicAdd((unsigned long long *)&hist[down >> kBinShift], (unsigned long long)(w | 1ull << 50));
+            for (int x = 0; x < View::N; x++)
+                if (v[x] >= low) add(kSharpDown, v[x] == m ? 1ull << (kCutBits - 1) : 0);
+        } else {  // every lane weighs, what is below `low` goes nowhere
+#pragma unroll
+            for (int x = 0; x < View::N; x++) {
+                if (x >= View::N - View::V && view.off == 0) continue;
+                double r;
+                const int k = unit.steps(v[x], r);
+                const uint64_t w = draw_value(k, r, kCutBits, tab);
+                if (v[x] >= low) add(-k, w);
+            }
         }
         __syncthreads();
         const size_t at = (row * P + p) * kBins;

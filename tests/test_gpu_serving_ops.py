@@ -696,3 +696,40 @@ def test_served_step_eager_and_replayed(be, tens):
         step()
         for a, b in zip(got, read()):
             assert np.array_equal(a, b)
+
+
+def test_two_lanes_at_once(be, tens):
+    """The three operators on both lanes in turn, each lane with its own work area and outputs: the results of one lane
+    alone."""
+    import rsv
+    rng = np.random.default_rng(23)
+    n, rows = 65529, 9
+    c = [Adapters(tens, np.random.default_rng(s), 130, 5, 16, [(520, 264)], "f16", "f32") for s in (1, 2)]
+    l = rng.standard_normal((rows, n)).astype(np.float32) * 3
+    f, u, logits = [FILTERS[i % 10] for i in range(rows)], rng.random(rows), tens(l)
+    t_f, t_u = tens(filters_of(f)), tens(u)
+    out = [(tens(n=rows, dtype=rsv.U32), tens(n=rows), tens(n=rows), tens(n=rsv.hip_lib().rsv_logits_work(n, rows)))
+           for _ in range(2)]
+    for a in c:
+        a.upload()
+    be.call("rsv_synchronize")
+    try:
+        for rep in range(4):
+            for lane in (0, 1):
+                be.call("rsv_lane_select", lane)
+                tok, logp, full, work = out[lane]
+                c[lane].call(be)
+                be.call("rsv_sample_rand_batch", logits, tok, n, t_f, t_u, logp, work, rows)
+                be.call("rsv_token_logprobs", logits, tok, n, full, NONE, work, rows)
+        for lane in (0, 1):
+            be.call("rsv_lane_select", lane)
+            be.call("rsv_synchronize")
+    finally:
+        be.call("rsv_lane_select", 0)
+    for lane in (0, 1):
+        c[lane].check(be)
+    a, b = [[be.get(o[0], rows, rsv.U32), be.get(o[1], rows), be.get(o[2], rows)] for o in out]
+    assert all(np.array_equal(x, y) for x, y in zip(a, b))
+    for r in range(rows):
+        want, lp = draw64(l[r], *[np.float32(v) if j != 1 else v for j, v in enumerate(f[r])], np.float32(u[r]))
+        assert a[0][r] == want and abs(a[1][r] - lp) <= 2 * U * abs(lp) + 1e-9

@@ -459,7 +459,10 @@ __global__ __launch_bounds__(kDownThreads) void k_adapter_down(AdapterJobs J, in
 
 // The two launches are bound by memory: r/k/v of 4096 rows (fp16 x, fp32 y and
 // out in place) move 325 MB in 18.4 + 46.4 us (5.0 TB/s; a copy reaches 5.1);
-// 517 rows of k = 10240 take 9.3 + 8.7, mostly ramp and tail.
+// 517 rows of k = 10240 take 9.3 + 8.7, mostly ramp and tail.  Windows of many
+// adapters with a row each keep too few bytes in flight (256 rows of 256
+// adapters, r/k/v: 72 us, 1.7 TB/s); two to four times the slots below make
+// that 73 to 76.
 //
 // The outputs of a window's rows in a piece of n.  h's slices are added in
 // order and split into two fp16 numbers, hi + lo, after each row is scaled by

@@ -60,12 +60,12 @@ __device__ __forceinline__ void lg_unpack(uint4 q, float (&v)[F16 ? 8 : 4]) {
 //   narrowed to one key, the draw's piece follows from the pieces' kept sums and
 //   the token from that piece alone.
 //
-// Bounds.  Many rows without cuts stream: 256 rows of 65536 fp32 logits take 25
-// us in the first launch (2.7 TB/s; the rest is 64-bit float work) and 6.5 in
+// Bounds.  Many rows without cuts stream: 256 rows of 65536 fp32 logits take 21
+// us in the first launch (3.2 TB/s; the rest is 64-bit float work) and 6.6 in
 // the second.  Rows with cuts are bound by the second launch's chain of reads,
 // barriers and LDS round trips on one CU: of one peaked row's 13 us, 3 are the
 // settings, the pieces and the table, 3 the bin, 6 the listing, 2 the rest; 64
-// mixed rows take 8.4 + 22.  A piece's own list of its largest tokens, made by
+// mixed rows take 7.6 + 22.  A piece's own list of its largest tokens, made by
 // the first launch, saved 5 us of listing and cost 1.6 there and 1 to 5 in rows
 // that it did not settle.  256 threads: what all waves do alike costs a SIMD's
 // issue slots once a wave, and 16 waves a block took four times as long for it.
